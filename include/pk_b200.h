@@ -225,6 +225,117 @@ typedef struct pk_tdt_desc {
 } pk_tdt_desc;
 int pk_tdt_decode(pk_device* device, const pk_tdt_desc* desc, pk_stream stream);
 
+/* ------------------------------------------------------------- scoring
+ * A decoder's last steps, from a block's output to a scored answer.  No
+ * counterparts in the reference, which returns token ids alone.  No entry
+ * point here holds a workspace: calls on different streams may overlap, and
+ * captured graphs may run side by side.  Each leaves the calling thread's
+ * current device as it was.
+ *
+ * Token scores: for every row of logits x [columns], with the softmax p:
+ *   log_probs   log p[target]      log_sums   log sum exp x
+ *   entropies   -sum p log p       top_ids / top_log_probs  the top_k best
+ * columns by value, then by the lower index.  Any output may be NULL
+ * (log_probs needs targets).  Masked columns are -inf and have probability 0;
+ * a row of -inf alone scores -inf everywhere, with entropy 0 and the lowest
+ * ids.  A row with NaN or +inf scores NaN (its ids rank NaN as -inf); a target
+ * id >= columns scores NaN. */
+typedef struct pk_token_scores_desc {
+  int precision;             /* of the logits: PK_FP16 or PK_FP32 */
+  int top_k;                 /* 0..32, at most columns */
+  int64_t rows, columns;
+  int64_t row_stride;        /* elements between rows, >= columns */
+  const void* logits;        /* device; element-aligned */
+  const uint32_t* targets;   /* device u32 [slots] or NULL */
+  const uint32_t* row_count; /* device u32 [1] or NULL: rows at and behind it are left out */
+  const uint32_t* row_map;   /* device u32 [rows] or NULL: row r takes targets and outputs at slot row_map[r] */
+  int64_t slots;             /* entries of targets and outputs; rows whose slot is outside are left out */
+  float* log_probs;          /* device f32 [slots] */
+  float* log_sums;
+  float* entropies;
+  uint32_t* top_ids;         /* device u32 [slots, top_k] */
+  float* top_log_probs;      /* device f32 [slots, top_k] */
+} pk_token_scores_desc;
+int pk_token_scores(pk_device* device, const pk_token_scores_desc* desc, pk_stream stream);
+
+/* The norms before and after a block with its gate and residual scale:
+ *   u = post(block), y = input + residual_scale * gate * u, h = pre(y)
+ * where post and pre are PK_NORM_*; y (output) and h (normalized) are each
+ * rounded once, h from the unrounded y.  LayerNorm has gamma and beta, RMS
+ * norm gamma alone.  gate: NULL, or f32 [ceil(rows / gate_rows), channels]
+ * (one row for each gate_rows rows; gate_rows 0: one row for all).  output
+ * and normalized may take the place of input or block (exactly), not of each
+ * other. */
+enum { PK_NORM_NONE = 0, PK_NORM_LAYER = 1, PK_NORM_RMS = 2 };
+typedef struct pk_residual_norm_desc {
+  int precision;             /* PK_FP16 or PK_FP32: input, block, output, normalized */
+  int post, pre;             /* PK_NORM_* */
+  int64_t rows;
+  int64_t channels;          /* a multiple of 4, at most 32768 */
+  int64_t gate_rows;
+  float residual_scale;
+  float epsilon;
+  const void* input;         /* device [rows, channels]: the residual stream */
+  const void* block;         /* device [rows, channels]: the block's output */
+  const float* post_gamma;   /* device f32 [channels] */
+  const float* post_beta;
+  const float* pre_gamma;
+  const float* pre_beta;
+  const float* gate;
+  void* output;              /* device [rows, channels] */
+  void* normalized;          /* device [rows, channels]; NULL exactly when pre is PK_NORM_NONE */
+} pk_residual_norm_desc;
+int pk_residual_norm(pk_device* device, const pk_residual_norm_desc* desc, pk_stream stream);
+
+/* A few rows times a matrix held in 4 bits, the decode form of the palette
+ * GEMM: C = epilogue(A . W), W[k, n] = (code[k, n] - 8) * scales[k / group, n].
+ * The scale multiplies the group's f32 sum.  Epilogue as in pk_gemm_desc; bias
+ * and residual are exclusive.  Codes lie in tiles of 16 outputs x 128 inputs
+ * ("n16-k128-lane-major-int4-u32"): u32 [ceil(N / 16)][ceil(K / 128)][2][32][4],
+ * where word i of lane l in half h holds, lowest bits first, the codes of
+ * inputs 128 kt + 32 i + 8 (l % 4) + 0..7 of output 16 nt + 8 h + l / 4; places
+ * outside the matrix hold code 8. */
+typedef struct pk_int4_gemv_desc {
+  int precision;             /* PK_FP16: A/C/residual/scales f16; PK_FP32: all f32 */
+  int64_t rows;              /* 1..64 */
+  int64_t inner;             /* K, a multiple of 32 */
+  int64_t columns;           /* N */
+  int64_t group;             /* inputs per scale: 32, 64 or a multiple of 128; divides K */
+  int activation;            /* PK_ACT_* */
+  float residual_scale;
+  const float* bias;         /* device f32 [N] or NULL */
+  const void* residual;      /* device [rows, N] or NULL: C = residual + residual_scale * value; may be C */
+  const void* a;             /* device [rows, K], 16-byte aligned */
+  const uint32_t* codes;     /* device, 16-byte aligned */
+  const void* scales;        /* device [K / group, N] */
+  void* c;                   /* device [rows, N] */
+} pk_int4_gemv_desc;
+int pk_int4_gemv(pk_device* device, const pk_int4_gemv_desc* desc, pk_stream stream);
+
+/* The joint of the emitted tokens of a batch of windows, ragged:
+ *   hidden = max(encoder_projected[w, joint_frames[w, u]] + predictor[w, u], 0)
+ *   logits[r] = hidden . weight + bias
+ * for u < min(counts[w], max_tokens), rows in order of (w, u); FP16 rounds
+ * hidden to f16, as the decoder does.  row_map[r] = w * max_tokens + u and
+ * row_count are what pk_token_scores takes.  Rows behind the last are left as
+ * they are.  Frames >= frames are read as frames - 1. */
+typedef struct pk_joint_logits_desc {
+  int precision;                 /* PK_FP16: encoder, weight, logits f16; PK_FP32: f32 */
+  int batch, frames, max_tokens;
+  int64_t inner;                 /* a multiple of 32 */
+  int64_t columns;               /* a multiple of 8 */
+  const void* encoder_projected; /* device [batch, frames, inner] */
+  const float* predictor;        /* device f32 [batch, max_tokens, inner] */
+  const uint32_t* joint_frames;  /* device u32 [batch, max_tokens] */
+  const uint32_t* counts;        /* device u32 [batch] */
+  const void* weight;            /* device [inner, columns] (k-by-output) */
+  const float* bias;             /* device f32 [columns] or NULL */
+  void* logits;                  /* device [batch * max_tokens, columns]; all of these 16-byte aligned */
+  uint32_t* row_map;             /* device u32 [batch * max_tokens] */
+  uint32_t* row_count;           /* device u32 [1] */
+} pk_joint_logits_desc;
+int pk_joint_logits(pk_device* device, const pk_joint_logits_desc* desc, pk_stream stream);
+
 /* ------------------------------------------------------------ model + graph
  * One named tensor of a weight package (ParakeetTensorRecord,
  * src/model/manifest.ts; runtime layouts src/model/runtime-plan.ts:26-37). */

@@ -21,6 +21,7 @@ FP16, FP32 = 0, 1
 ACT = {"none": 0, "silu": 1, "relu": 2}
 LAYOUT_ROW_MAJOR, LAYOUT_TILE_MAJOR = 0, 1
 DTYPE_F16, DTYPE_F32, DTYPE_U32 = 0, 1, 2
+NORM = {"none": 0, "layer": 1, "rms": 2}
 
 # Every symbol include/pk_b200.h declares.
 EXPORTED = (
@@ -34,7 +35,7 @@ EXPORTED = (
     "pk_debug_set_gemm_tile", "pk_debug_set_attention_route", "pk_debug_set_decoder_route",
     "pk_debug_wait_probe", "pk_stitch_create", "pk_stitch_destroy", "pk_stitch_append", "pk_stitch_append_tdt",
     "pk_stitch_extend", "pk_stitch_counts", "pk_stitch_read", "pk_stitch_read_run",
-    "pk_debug_set_reference_arithmetic",
+    "pk_debug_set_reference_arithmetic", "pk_token_scores", "pk_residual_norm", "pk_int4_gemv", "pk_joint_logits",
 )
 STITCH_COLLECT_TRACE, STITCH_RECORD_RUN = 1, 2
 
@@ -86,6 +87,38 @@ class TdtDesc(ctypes.Structure):
         "head_weight", "head_bias", "tokens", "token_frames", "token_durations", "metadata")]
 
 
+class TokenScoresDesc(ctypes.Structure):
+    _fields_ = [
+        ("precision", ctypes.c_int), ("top_k", ctypes.c_int), ("rows", ctypes.c_int64), ("columns", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64), ("logits", ctypes.c_void_p), ("targets", ctypes.c_void_p),
+        ("row_count", ctypes.c_void_p), ("row_map", ctypes.c_void_p), ("slots", ctypes.c_int64),
+    ] + [(n, ctypes.c_void_p) for n in ("log_probs", "log_sums", "entropies", "top_ids", "top_log_probs")]
+
+
+class ResidualNormDesc(ctypes.Structure):
+    _fields_ = [
+        ("precision", ctypes.c_int), ("post", ctypes.c_int), ("pre", ctypes.c_int), ("rows", ctypes.c_int64),
+        ("channels", ctypes.c_int64), ("gate_rows", ctypes.c_int64), ("residual_scale", ctypes.c_float),
+        ("epsilon", ctypes.c_float),
+    ] + [(n, ctypes.c_void_p) for n in ("input", "block", "post_gamma", "post_beta", "pre_gamma", "pre_beta", "gate",
+                                        "output", "normalized")]
+
+
+class Int4GemvDesc(ctypes.Structure):
+    _fields_ = [
+        ("precision", ctypes.c_int), ("rows", ctypes.c_int64), ("inner", ctypes.c_int64), ("columns", ctypes.c_int64),
+        ("group", ctypes.c_int64), ("activation", ctypes.c_int), ("residual_scale", ctypes.c_float),
+    ] + [(n, ctypes.c_void_p) for n in ("bias", "residual", "a", "codes", "scales", "c")]
+
+
+class JointLogitsDesc(ctypes.Structure):
+    _fields_ = [
+        ("precision", ctypes.c_int), ("batch", ctypes.c_int), ("frames", ctypes.c_int), ("max_tokens", ctypes.c_int),
+        ("inner", ctypes.c_int64), ("columns", ctypes.c_int64),
+    ] + [(n, ctypes.c_void_p) for n in ("encoder_projected", "predictor", "joint_frames", "counts", "weight", "bias",
+                                        "logits", "row_map", "row_count")]
+
+
 class TensorDesc(ctypes.Structure):
     _fields_ = [
         ("name", ctypes.c_char_p), ("dtype", ctypes.c_int), ("ndim", ctypes.c_int),
@@ -125,6 +158,10 @@ def load() -> ctypes.CDLL:
             "pk_subsampling_time_mask": [vp, i32, i32, i32, i32, i32, vp, vp, i32, vp],
             "pk_tdt_decode": [vp, ctypes.POINTER(TdtDesc), vp],
             "pk_logmel": [vp, i32, i32, vp, vp, vp, vp],
+            "pk_token_scores": [vp, ctypes.POINTER(TokenScoresDesc), vp],
+            "pk_residual_norm": [vp, ctypes.POINTER(ResidualNormDesc), vp],
+            "pk_int4_gemv": [vp, ctypes.POINTER(Int4GemvDesc), vp],
+            "pk_joint_logits": [vp, ctypes.POINTER(JointLogitsDesc), vp],
             "pk_weights_upload": [vp, ctypes.POINTER(TensorDesc), i32, ctypes.POINTER(vp)],
             "pk_weights_release": [vp],
             "pk_encoder_create": [vp, vp, i32, i32, ctypes.POINTER(vp)],

@@ -86,6 +86,23 @@ int validate_gemm(const GemmArgs& g) {
 
 static inline cudaStream_t as_stream(pk_stream s) { return static_cast<cudaStream_t>(s); }
 
+// Makes the handle's device current for the duration of a call.
+struct DeviceScope {
+  int before = -1;
+  int status = PK_OK;
+  explicit DeviceScope(const DeviceCtx& ctx) {
+    int now = 0;
+    cudaError_t e = cudaGetDevice(&now);
+    if (e == cudaSuccess && now != ctx.ordinal && (e = cudaSetDevice(ctx.ordinal)) == cudaSuccess) before = now;
+    if (e != cudaSuccess) status = cuda_error(e, "cudaSetDevice");
+  }
+  ~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+static inline bool misaligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
 }  // namespace pk
 
 using namespace pk;
@@ -354,6 +371,100 @@ int pk_subsampling_time_mask(pk_device* device, int precision, int batch, int he
   cudaSetDevice(device->ctx.ordinal);
   return launch_subsampling_time_mask(precision, batch, height, width, channels, values, feature_lengths, steps,
                                       as_stream(stream));
+}
+
+int pk_token_scores(pk_device* device, const pk_token_scores_desc* d, pk_stream stream) {
+  if (!device || !d || !d->logits) return set_error(PK_E_INVALID, "null argument");
+  if (d->precision != PK_FP16 && d->precision != PK_FP32) return set_error(PK_E_INVALID, "unknown precision");
+  if (d->rows <= 0 || d->rows > (int64_t)1 << 30 || d->columns <= 0 || d->columns > (int64_t)1 << 30)
+    return set_error(PK_E_SHAPE, "token scores take 1..2^30 rows and columns");
+  if (d->row_stride < d->columns) return set_error(PK_E_SHAPE, "row stride %lld is below the %lld columns",
+                                                   (long long)d->row_stride, (long long)d->columns);
+  if (d->top_k < 0 || d->top_k > 32 || d->top_k > d->columns)
+    return set_error(PK_E_SHAPE, "top_k must be in [0, 32] and at most the columns, got %d", d->top_k);
+  if (d->slots < (d->row_map ? 1 : d->rows)) return set_error(PK_E_SHAPE, "outputs hold %lld of %lld rows",
+                                                              (long long)d->slots, (long long)d->rows);
+  if (d->log_probs && !d->targets) return set_error(PK_E_INVALID, "log probabilities need target ids");
+  if (!d->log_probs && !d->log_sums && !d->entropies && !d->top_ids && !d->top_log_probs)
+    return set_error(PK_E_INVALID, "token scores without an output");
+  if (misaligned(d->logits, d->precision == PK_FP16 ? 2 : 4)) return set_error(PK_E_LAYOUT, "logits are not element-aligned");
+  DeviceScope scope(device->ctx);
+  if (scope.status != PK_OK) return scope.status;
+  return launch_token_scores(device->ctx, *d, as_stream(stream));
+}
+
+int pk_residual_norm(pk_device* device, const pk_residual_norm_desc* d, pk_stream stream) {
+  if (!device || !d || !d->input || !d->block || !d->output) return set_error(PK_E_INVALID, "null argument");
+  if (d->precision != PK_FP16 && d->precision != PK_FP32) return set_error(PK_E_INVALID, "unknown precision");
+  if (d->rows <= 0 || d->rows > (int64_t)1 << 30 || d->channels <= 0 || d->channels % 4 != 0 || d->channels > 32768)
+    return set_error(PK_E_SHAPE, "residual norm rows must be in [1, 2^30] and channels a multiple of 4 in [4, 32768]");
+  if (d->gate_rows < 0) return set_error(PK_E_SHAPE, "gate rows must not be negative");
+  const struct { int kind; const float* gamma; const float* beta; const char* name; } norms[] = {
+      {d->post, d->post_gamma, d->post_beta, "post"}, {d->pre, d->pre_gamma, d->pre_beta, "pre"}};
+  for (const auto& n : norms) {
+    if (n.kind < PK_NORM_NONE || n.kind > PK_NORM_RMS) return set_error(PK_E_INVALID, "unknown %s norm %d", n.name, n.kind);
+    if ((n.gamma != nullptr) != (n.kind != PK_NORM_NONE) || (n.beta != nullptr) != (n.kind == PK_NORM_LAYER))
+      return set_error(PK_E_INVALID, "the %s norm takes %s", n.name,
+                       n.kind == PK_NORM_LAYER ? "gamma and beta" : n.kind == PK_NORM_RMS ? "gamma alone" : "no parameters");
+  }
+  if ((d->normalized != nullptr) != (d->pre != PK_NORM_NONE))
+    return set_error(PK_E_INVALID, "a normalized output and a pre norm belong together");
+  if (d->normalized == d->output) return set_error(PK_E_INVALID, "output and normalized are the same buffer");
+  const uintptr_t es = d->precision == PK_FP16 ? 2 : 4;
+  const void* data[] = {d->input, d->block, d->output, d->normalized};
+  for (const void* q : data)
+    if (misaligned(q, es)) return set_error(PK_E_LAYOUT, "residual norm operands are not element-aligned");
+  // A row is read whole before it is written: exact aliases are safe, shifted ones are not.
+  const size_t bytes = (size_t)d->rows * d->channels * es;
+  const void* outs[] = {d->output, d->normalized};
+  for (const void* o : outs)
+    for (const void* i : data) {
+      const uintptr_t a = reinterpret_cast<uintptr_t>(o), b = reinterpret_cast<uintptr_t>(i);
+      if (o && i && a != b && a < b + bytes && b < a + bytes)
+        return set_error(PK_E_INVALID, "residual norm buffers overlap without being the same");
+    }
+  DeviceScope scope(device->ctx);
+  if (scope.status != PK_OK) return scope.status;
+  return launch_residual_norm(*d, as_stream(stream));
+}
+
+int pk_int4_gemv(pk_device* device, const pk_int4_gemv_desc* d, pk_stream stream) {
+  if (!device || !d || !d->a || !d->codes || !d->scales || !d->c) return set_error(PK_E_INVALID, "null argument");
+  if (d->precision != PK_FP16 && d->precision != PK_FP32) return set_error(PK_E_INVALID, "unknown precision");
+  if (d->rows < 1 || d->rows > 64) return set_error(PK_E_SHAPE, "int4 products take 1..64 rows, got %lld", (long long)d->rows);
+  if (d->inner <= 0 || d->inner % 32 != 0 || d->inner > (1 << 20) || d->columns <= 0 || d->columns > (1 << 22))
+    return set_error(PK_E_SHAPE, "Unsupported int4 shape: K=%lld N=%lld (needs K%%32==0)", (long long)d->inner,
+                     (long long)d->columns);
+  if (d->group <= 0 || d->inner % d->group != 0 || (d->group != 32 && d->group != 64 && d->group % 128 != 0))
+    return set_error(PK_E_LAYOUT, "int4 groups are 32, 64 or a multiple of 128 inputs and divide K, got %lld of %lld",
+                     (long long)d->group, (long long)d->inner);
+  if (d->activation < PK_ACT_NONE || d->activation > PK_ACT_RELU) return set_error(PK_E_INVALID, "unknown activation %d", d->activation);
+  if (d->bias && d->residual) return set_error(PK_E_SIGNATURE, "cannot fuse bias and residual together");
+  if (misaligned(d->a, 16) || misaligned(d->codes, 16)) return set_error(PK_E_LAYOUT, "int4 rows and codes must be 16-byte aligned");
+  DeviceScope scope(device->ctx);
+  if (scope.status != PK_OK) return scope.status;
+  return launch_int4_gemv(device->ctx, *d, as_stream(stream));
+}
+
+int pk_joint_logits(pk_device* device, const pk_joint_logits_desc* d, pk_stream stream) {
+  if (!device || !d) return set_error(PK_E_INVALID, "null argument");
+  const void* ptrs[] = {d->encoder_projected, d->predictor, d->weight, d->logits, d->joint_frames, d->counts, d->row_map, d->row_count};
+  for (const void* q : ptrs)
+    if (!q) return set_error(PK_E_INVALID, "joint pointer is null");
+  if (d->precision != PK_FP16 && d->precision != PK_FP32) return set_error(PK_E_INVALID, "unknown precision");
+  if (d->batch <= 0 || d->batch > 65535 || d->frames <= 0 || d->max_tokens <= 0 ||
+      (int64_t)d->batch * d->max_tokens > (int64_t)1 << 30 || (int64_t)d->batch * d->frames > (int64_t)1 << 30)
+    return set_error(PK_E_SHAPE, "invalid joint batch geometry");
+  if (d->inner <= 0 || d->inner % 32 != 0 || d->inner > (1 << 20) || d->columns <= 0 || d->columns % 8 != 0 ||
+      d->columns > (1 << 20))
+    return set_error(PK_E_SHAPE, "Unsupported joint shape: K=%lld N=%lld (needs K%%32==0, N%%8==0)", (long long)d->inner,
+                     (long long)d->columns);
+  const void* aligned16[] = {d->encoder_projected, d->predictor, d->weight, d->logits, d->bias};
+  for (const void* q : aligned16)
+    if (misaligned(q, 16)) return set_error(PK_E_LAYOUT, "joint operands must be 16-byte aligned");
+  DeviceScope scope(device->ctx);
+  if (scope.status != PK_OK) return scope.status;
+  return launch_joint_logits(device->ctx, *d, as_stream(stream));
 }
 
 }  // extern "C"

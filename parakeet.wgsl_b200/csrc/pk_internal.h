@@ -117,6 +117,12 @@ int launch_subsampling_depthwise(int precision, int batch, int ih, int iw, int c
 int launch_subsampling_time_mask(int precision, int batch, int height, int width, int channels, void* values,
                                  const uint32_t* feature_lengths, int steps, cudaStream_t stream);
 
+// Scoring operators (token_scores.cu, residual_norm.cu, int4_gemv.cu, joint_logits.cu).
+int launch_token_scores(const DeviceCtx& dev, const pk_token_scores_desc& d, cudaStream_t stream);
+int launch_residual_norm(const pk_residual_norm_desc& d, cudaStream_t stream);
+int launch_int4_gemv(const DeviceCtx& dev, const pk_int4_gemv_desc& d, cudaStream_t stream);
+int launch_joint_logits(const DeviceCtx& dev, const pk_joint_logits_desc& d, cudaStream_t stream);
+
 int launch_tdt_decode(const DeviceCtx& dev, const pk_tdt_desc& d, cudaStream_t stream);
 // Resident FP16 decoder (all windows in lockstep on 128 co-resident CTAs);
 // returns PK_E_SHAPE when it does not apply (then the cluster kernel runs).

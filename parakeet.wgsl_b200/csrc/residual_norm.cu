@@ -1,0 +1,286 @@
+// residual_norm.cu -- what stands between two blocks of a network, in one pass:
+//
+//   u = post(block)                     the norm after the block
+//   y = input + scale * gate * u        its gate and residual scale; the residual stream
+//   h = pre(y)                          the next block's norm
+//
+// post and pre are LayerNorm ((v - mean) rstd gamma + beta), RMS norm
+// (v rrms gamma) or absent; the gate is absent, one row of channels, or one
+// row for every `gate_rows` rows.  y and h are each rounded once: h is the
+// norm of y before its rounding.  Means and variances are f32, the variance
+// from the centred values (a second sum over registers costs no memory, and
+// E[v^2] - mean^2 loses what a large mean hides).
+//
+// Bound by memory: two reads and two writes of every element, nothing in
+// between reaches memory.  A row lives in the registers of 32 to 1024 threads;
+// all its loads are issued before the first is used, and gamma, beta and gate
+// come from L1 after the first rows.
+#include "pk_common.cuh"
+#include "pk_internal.h"
+
+namespace pk {
+namespace {
+
+struct RnParams {
+  const void* x;
+  const void* f;
+  const float* post_gamma;
+  const float* post_beta;
+  const float* pre_gamma;
+  const float* pre_beta;
+  const float* gate;
+  void* y;
+  void* h;
+  int64_t rows, gate_rows;
+  int channels, post, pre;
+  float scale, eps;
+};
+
+// VEC elements of T as one load or store.
+template <int BYTES>
+struct RnWord;
+template <>
+struct RnWord<16> { using type = uint4; };
+template <>
+struct RnWord<8> { using type = uint2; };
+template <>
+struct RnWord<4> { using type = uint32_t; };
+template <>
+struct RnWord<2> { using type = uint16_t; };
+
+template <typename T, int VEC>
+__device__ __forceinline__ void rn_unpack(const typename RnWord<VEC * sizeof(T)>::type& raw, float (&v)[VEC]) {
+  const T* e = reinterpret_cast<const T*>(&raw);
+  if constexpr (sizeof(T) == 2 && VEC > 1) {
+    const __half2* e2 = reinterpret_cast<const __half2*>(&raw);
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) {
+      const float2 f = __half22float2(e2[j]);
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = (float)e[j];
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ typename RnWord<VEC * sizeof(T)>::type rn_pack(const float (&v)[VEC]) {
+  typename RnWord<VEC * sizeof(T)>::type raw;
+  T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) e[j] = (T)v[j];
+  return raw;
+}
+template <int VEC>
+__device__ __forceinline__ void rn_params(const float* src, float (&v)[VEC]) {
+  if constexpr (VEC >= 4) {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 4) *reinterpret_cast<float4*>(v + j) = __ldg(reinterpret_cast<const float4*>(src + j));
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = __ldg(src + j);
+  }
+}
+
+// Sum over the G threads of a row.  Rows of more than a warp meet in shared
+// memory; `turn` alternates the two halves of `red`, so one barrier a sum is enough.
+template <int G>
+__device__ __forceinline__ float rn_sum(float v, float* red, int& turn) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (G > 32) {
+    float* mine = red + 32 * turn;
+    turn ^= 1;
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) mine[warp] = v;
+    __syncthreads();
+    const int w0 = (int)threadIdx.x / G * (G / 32);
+    v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < G / 32; ++w) v += mine[w0 + w];
+  }
+  return v;
+}
+
+// G threads per row, NV vectors of VEC elements per thread, blockDim / G rows per CTA.
+template <typename T, int VEC, int G, int NV>
+__global__ void __launch_bounds__(G > 256 ? G : 256) residual_norm_kernel(const RnParams p) {
+  pdl_entry();
+  using Word = typename RnWord<VEC * sizeof(T)>::type;
+  __shared__ float red[64];
+  int turn = 0;
+  const int t = threadIdx.x % G;
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / G) + threadIdx.x / G;
+  const bool live = row < p.rows;
+  const int C = p.channels;
+  const int words = C / VEC;
+  const Word* fx = reinterpret_cast<const Word*>(static_cast<const T*>(p.f) + (live ? row : 0) * C);
+  const Word* xx = reinterpret_cast<const Word*>(static_cast<const T*>(p.x) + (live ? row : 0) * C);
+  // With 1024 threads and more than 16 elements each, the residual's words do
+  // not fit beside the block's values: they are read when they are used.
+  constexpr bool EARLY = G < 1024 || VEC * NV <= 16;
+  Word fr[NV], xr[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (live && t + i * G < words) fr[i] = fx[t + i * G];
+  if constexpr (EARLY) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (live && t + i * G < words) xr[i] = xx[t + i * G];
+  }
+  float v[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (live && t + i * G < words) {
+      rn_unpack<T, VEC>(fr[i], v[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[i][j] = 0.0f;
+    }
+  }
+  const float inv = 1.0f / (float)C;
+  // Mean and 1 / deviation (RMS: 0 and 1 / root mean square) of the row in v.
+  auto stats = [&](int kind, float& mean, float& rstd) {
+    float s = 0.0f;
+    mean = 0.0f;
+    if (kind == PK_NORM_LAYER) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s += v[i][j];
+      mean = rn_sum<G>(s, red, turn) * inv;
+    }
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (t + i * G < words) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float d = v[i][j] - mean;
+          s = fmaf(d, d, s);
+        }
+      }
+    }
+    rstd = 1.0f / sqrtf(rn_sum<G>(s, red, turn) * inv + p.eps);
+  };
+  float mean = 0.0f, rstd = 1.0f;
+  if (p.post != PK_NORM_NONE) stats(p.post, mean, rstd);
+  const float* gate = p.gate ? p.gate + (p.gate_rows > 0 ? (live ? row : 0) / p.gate_rows : 0) * C : nullptr;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (t + i * G) * VEC;
+    if (live && t + i * G < words) {
+      float g[VEC], x[VEC];
+      if (p.post != PK_NORM_NONE) {
+        rn_params<VEC>(p.post_gamma + c, g);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] = (v[i][j] - mean) * rstd * g[j];
+        if (p.post == PK_NORM_LAYER) {
+          rn_params<VEC>(p.post_beta + c, g);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) v[i][j] += g[j];
+        }
+      }
+      if (gate) {
+        rn_params<VEC>(gate + c, g);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] *= g[j];
+      }
+      if constexpr (!EARLY) xr[i] = xx[t + i * G];
+      rn_unpack<T, VEC>(xr[i], x);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[i][j] = fmaf(p.scale, v[i][j], x[j]);
+    }
+  }
+  // The row is in registers, whole: where y or h takes the place of x or f,
+  // every thread has read its elements, and it writes only those.
+  Word* yo = reinterpret_cast<Word*>(static_cast<T*>(p.y) + (live ? row : 0) * C);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (live && t + i * G < words) yo[t + i * G] = rn_pack<T, VEC>(v[i]);
+  if (p.pre == PK_NORM_NONE) return;
+  stats(p.pre, mean, rstd);
+  Word* ho = reinterpret_cast<Word*>(static_cast<T*>(p.h) + (live ? row : 0) * C);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (t + i * G) * VEC;
+    if (live && t + i * G < words) {
+      float g[VEC];
+      rn_params<VEC>(p.pre_gamma + c, g);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[i][j] = (v[i][j] - mean) * rstd * g[j];
+      if (p.pre == PK_NORM_LAYER) {
+        rn_params<VEC>(p.pre_beta + c, g);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] += g[j];
+      }
+      ho[t + i * G] = rn_pack<T, VEC>(v[i]);
+    }
+  }
+}
+
+template <typename T, int VEC, int G, int NV>
+int launch_one(const RnParams& p, cudaStream_t stream) {
+  constexpr int threads = G > 256 ? G : 256;
+  const int64_t per = threads / G;
+  return cuda_error(launch_kernel(residual_norm_kernel<T, VEC, G, NV>, dim3((unsigned)((p.rows + per - 1) / per)),
+                                  dim3(threads), 0, stream, p),
+                    "residual_norm launch");
+}
+
+// The fewest threads that hold a row at NV vectors each.
+template <typename T, int VEC>
+int launch_vec(const RnParams& p, cudaStream_t stream) {
+  const int words = p.channels / VEC;
+  if (words <= 32) return launch_one<T, VEC, 32, 1>(p, stream);
+  if (words <= 128) return launch_one<T, VEC, 32, 4>(p, stream);
+  if (words <= 256) return launch_one<T, VEC, 64, 4>(p, stream);
+  if (words <= 512) return launch_one<T, VEC, 128, 4>(p, stream);
+  if (words <= 1024) return launch_one<T, VEC, 256, 4>(p, stream);
+  if (words <= 2048) return launch_one<T, VEC, 512, 4>(p, stream);
+  // Rows of at most 32768 channels: 4096 words of 8, 8192 of 4, 32768 single
+  // elements (a row whose start is not aligned).
+  if constexpr (VEC < 8) {
+    if (words > 4096) return launch_one<T, VEC, 1024, VEC == 1 ? 32 : 8>(p, stream);
+  }
+  return launch_one<T, VEC, 1024, 4>(p, stream);
+}
+
+template <typename T>
+int launch_typed(const RnParams& p, cudaStream_t stream) {
+  const uintptr_t data = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.f) |
+                         reinterpret_cast<uintptr_t>(p.y) | reinterpret_cast<uintptr_t>(p.h) |
+                         (uintptr_t)p.channels * sizeof(T);
+  const uintptr_t params = reinterpret_cast<uintptr_t>(p.post_gamma) | reinterpret_cast<uintptr_t>(p.post_beta) |
+                           reinterpret_cast<uintptr_t>(p.pre_gamma) | reinterpret_cast<uintptr_t>(p.pre_beta) |
+                           reinterpret_cast<uintptr_t>(p.gate);
+  if ((data & 15) == 0 && (params & 15) == 0) return launch_vec<T, 16 / sizeof(T)>(p, stream);
+  if (sizeof(T) == 2 && (data & 7) == 0 && (params & 15) == 0) return launch_vec<T, 8 / sizeof(T)>(p, stream);
+  return launch_vec<T, 1>(p, stream);
+}
+
+}  // namespace
+
+int launch_residual_norm(const pk_residual_norm_desc& d, cudaStream_t stream) {
+  RnParams p;
+  p.x = d.input;
+  p.f = d.block;
+  p.post_gamma = d.post_gamma;
+  p.post_beta = d.post_beta;
+  p.pre_gamma = d.pre_gamma;
+  p.pre_beta = d.pre_beta;
+  p.gate = d.gate;
+  p.y = d.output;
+  p.h = d.normalized;
+  p.rows = d.rows;
+  p.gate_rows = d.gate_rows;
+  p.channels = (int)d.channels;
+  p.post = d.post;
+  p.pre = d.pre;
+  p.scale = d.residual_scale;
+  p.eps = d.epsilon;
+  return d.precision == PK_FP16 ? launch_typed<__half>(p, stream) : launch_typed<float>(p, stream);
+}
+
+}  // namespace pk

@@ -658,6 +658,303 @@ class SubsamplingTimeMaskKernel:
         return disp
 
 
+# --------------------------------------------------------------------- scoring operators
+# A decoder's last steps, from a block's output to a scored answer.  They have
+# no counterparts in the reference, which returns token ids alone; they keep
+# the layer's shape (create -> create_dispatch -> encode -> destroy).  A
+# dispatch's pointers and sizes are fixed at creation, so encode is one C call.
+
+class _FixedDispatch(_Dispatch):
+    """A dispatch whose descriptor never changes; keeps its buffers alive."""
+
+    def __init__(self, label: str, device: Device, entry: str, desc, buffers):
+        super().__init__(label)
+        self._device, self._entry = device, getattr(_lib.load(), entry)
+        self._desc, self._ref, self._buffers = desc, ctypes.byref(desc), buffers
+
+    def encode(self, stream=None, timestamp_writes=None) -> None:
+        """Launches on `stream` (default: the current stream of the kernel's device)."""
+        if self._destroyed or self._device.handle is None:
+            raise ParakeetError(f"{self.label} was destroyed")
+        if stream is None:
+            stream = torch.cuda.current_stream(self._device.ordinal).cuda_stream
+        else:
+            stream = _stream_handle(stream)
+        status = self._entry(self._device.handle, self._ref, stream)
+        if status:
+            _lib.check(status)
+
+
+def _operand(d: dict, key: str, dtype, count: int, device: Device, optional: bool = False):
+    """The buffer d[key]: a contiguous CUDA tensor (or GpuTensor) on the
+    kernel's device with at least `count` elements of `dtype`."""
+    t = d.get(key)
+    if t is None:
+        if optional:
+            return None
+        raise ParakeetError(f"{d.get('label', 'dispatch')} needs {key}")
+    if isinstance(t, GpuTensor):
+        t = t.tensor
+    if not t.is_cuda or not t.is_contiguous() or t.device.index != device.ordinal:
+        raise ParakeetError(f"{d.get('label', 'dispatch')} {key} must be a contiguous tensor on cuda:{device.ordinal}")
+    allowed = dtype if isinstance(dtype, tuple) else (dtype,)
+    if t.dtype not in allowed:
+        raise ParakeetError(f"{d.get('label', 'dispatch')} {key} must be {allowed[0]}, got {t.dtype}")
+    if t.numel() < count:
+        raise RangeError(f"{d.get('label', 'dispatch')} {key} needs {count} elements, got {t.numel()}")
+    return t
+
+
+def _address(t, first: int = 0) -> int | None:
+    return None if t is None else t.data_ptr() + first * t.element_size()
+
+
+def _sizes(d: dict, **least) -> list[int]:
+    out = []
+    for key, low in least.items():
+        v = d[key]
+        if not isinstance(v, int) or isinstance(v, bool) or v < low:
+            raise RangeError(f"{d.get('label', 'dispatch')} {key} must be an integer of at least {low}")
+        out.append(v)
+    return out
+
+
+def _ids():
+    return (torch.int32, torch.uint32)
+
+
+class TokenScoresKernel:
+    """Log probability of a given token, log of the normaliser, entropy and the
+    best alternatives of every row of logits (pk_token_scores)."""
+
+    def __init__(self, device: Device, profile: str):
+        self.device, self.profile = device, profile
+
+    @staticmethod
+    def create(device: Device, arena=None, capacity: int = 0, profile: str = "fp16") -> "TokenScoresKernel":
+        """profile: the scalar of the logits."""
+        _precision(profile)
+        return TokenScoresKernel(device, profile)
+
+    def create_dispatch(self, d: dict) -> _Dispatch:
+        """d: label, logits, rows, columns, row_stride=columns, first_column=0 (the row's
+        first element in the buffer's rows), top_k=0, and the outputs wanted: log_probs (with
+        targets), log_sums, entropies (f32 [slots]), top_ids (u32 [slots, top_k]), top_log_probs
+        (f32 [slots, top_k]).  row_count (u32 [1]) and row_map (u32 [rows]), both on the device,
+        restrict and scatter the rows as pk_joint_logits leaves them; slots (default: rows) is
+        the number of entries of targets and outputs."""
+        label = d["label"]
+        rows, columns = _sizes(d, rows=1, columns=1)
+        opt = {"row_stride": columns, "first_column": 0, "top_k": 0, "slots": rows, **d}
+        stride, first, k, slots = _sizes(opt, row_stride=1, first_column=0, top_k=0, slots=1)
+        if first + columns > stride:
+            raise RangeError(f"{label} rows of {columns} columns from {first} do not fit a stride of {stride}")
+        if k > 32 or k > columns:
+            raise RangeError(f"{label} top_k must be in [0, 32] and at most {columns}, got {k}")
+        if "row_map" not in d and slots < rows:
+            raise RangeError(f"{label} outputs hold {slots} of {rows} rows")
+        f32 = torch.float32
+        logits = _operand(d, "logits", _scalar_dtype(self.profile), (rows - 1) * stride + first + columns, self.device)
+        dev = self.device
+        targets = _operand(d, "targets", _ids(), slots, dev, optional="log_probs" not in d)
+        outs = {n: _operand(d, n, f32, slots, dev, optional=True) for n in ("log_probs", "log_sums", "entropies")}
+        outs["top_ids"] = _operand(d, "top_ids", _ids(), slots * k, dev, optional=True)
+        outs["top_log_probs"] = _operand(d, "top_log_probs", f32, slots * k, dev, optional=True)
+        if all(t is None for t in outs.values()):
+            raise ParakeetError(f"{label} has no output")
+        count = _operand(d, "row_count", _ids(), 1, dev, optional=True)
+        rmap = _operand(d, "row_map", _ids(), rows, dev, optional=True)
+        if k == 0:
+            outs["top_ids"] = outs["top_log_probs"] = None
+            if all(t is None for t in outs.values()):
+                raise ParakeetError(f"{label} has no output")
+        desc = _lib.TokenScoresDesc(_precision(self.profile), k, rows, columns, stride, _address(logits, first),
+                                    _address(targets), _address(count), _address(rmap), slots,
+                                    *[_address(outs[n]) for n in ("log_probs", "log_sums", "entropies", "top_ids",
+                                                                  "top_log_probs")])
+        disp = _FixedDispatch(label, dev, "pk_token_scores", desc, (logits, targets, count, rmap, outs))
+        disp.output = outs
+        return disp
+
+
+class ResidualNormKernel:
+    """The norms before and after a block with its gate and residual scale (pk_residual_norm):
+    u = post(block), y = input + residual_scale * gate * u, h = pre(y)."""
+
+    def __init__(self, device: Device, profile: str):
+        self.device, self.profile = device, profile
+
+    @staticmethod
+    def create(device: Device, arena=None, capacity: int = 0, profile: str = "fp16") -> "ResidualNormKernel":
+        _precision(profile)
+        return ResidualNormKernel(device, profile)
+
+    def create_dispatch(self, d: dict) -> _Dispatch:
+        """d: label, input, block, output (y), normalized (h, with a pre norm), rows, channels,
+        post="none", pre="none" ("none" | "layer" | "rms") with post_gamma / post_beta / pre_gamma /
+        pre_beta (f32 [channels]; beta with "layer" alone), gate (f32 [ceil(rows / gate_rows),
+        channels]; gate_rows 0: one row for all), residual_scale=1.0, epsilon=1e-5.  output and
+        normalized may be input or block themselves."""
+        label, dev = d["label"], self.device
+        rows, channels = _sizes(d, rows=1, channels=1)
+        (gate_rows,) = _sizes({"gate_rows": 0, **d}, gate_rows=0)
+        if channels % 4 or channels > 32768:
+            raise RangeError(f"Unsupported residual norm shape for {label}")
+        kinds = [d.get("post", "none"), d.get("pre", "none")]
+        for at, kind in zip(("post", "pre"), kinds):
+            if kind not in _lib.NORM:
+                raise ParakeetError(f"{label} has an unknown {at} norm {kind!r}")
+            given = tuple(d.get(f"{at}_{n}") is not None for n in ("gamma", "beta"))
+            if given != {"none": (False, False), "rms": (True, False), "layer": (True, True)}[kind]:
+                raise ParakeetError(f"{label} {at} norm {kind!r} takes "
+                                    + {"none": "no parameters", "rms": "gamma alone", "layer": "gamma and beta"}[kind])
+        if (d.get("normalized") is not None) != (kinds[1] != "none"):
+            raise ParakeetError(f"{label} needs a normalized output exactly with a pre norm")
+        scalar, f32, n = _scalar_dtype(self.profile), torch.float32, rows * channels
+        data = [_operand(d, key, scalar, n, dev, optional=key == "normalized")
+                for key in ("input", "block", "output", "normalized")]
+        params = [_operand(d, key, f32, channels, dev, optional=True)
+                  for key in ("post_gamma", "post_beta", "pre_gamma", "pre_beta")]
+        groups = 1 if gate_rows == 0 else -(-rows // gate_rows)
+        gate = _operand(d, "gate", f32, groups * channels, dev, optional=True)
+        desc = _lib.ResidualNormDesc(_precision(self.profile), _lib.NORM[kinds[0]], _lib.NORM[kinds[1]], rows, channels,
+                                     gate_rows, float(d.get("residual_scale", 1.0)), float(d.get("epsilon", 1e-5)),
+                                     *[_address(t) for t in (data[0], data[1], *params, gate, data[2], data[3])])
+        disp = _FixedDispatch(label, dev, "pk_residual_norm", desc, (data, params, gate))
+        disp.output, disp.normalized = d["output"], d.get("normalized")
+        return disp
+
+
+@dataclass
+class Int4Weight:
+    """A [K, N] weight in 4 bits with a scale per `group` inputs and output, laid out for
+    pk_int4_gemv: W[k, n] = (code - 8) * scales[k // group, n]."""
+    inner: int
+    columns: int
+    group: int
+    codes: GpuTensor
+    scales: GpuTensor
+
+    @staticmethod
+    def from_words(words, scales, inner: int, group: int, name: str = "int4") -> "Int4Weight":
+        """words: CUDA int32 / uint32 [N, K / 8] (rp.INT4_LAYOUT), scales: CUDA f16 or f32
+        [K / group, N].  The re-laid codes are a copy; the scales are used as they are."""
+        columns = int(words.shape[0])
+        try:
+            rp.check_int4_geometry(inner, columns, group)
+        except ValueError as e:
+            raise RangeError(str(e)) from None
+        if tuple(words.shape) != (columns, inner // 8) or words.dtype not in _ids():
+            raise ParakeetError(f"{name} codes must be int32 or uint32 [{columns},{inner // 8}]")
+        if tuple(scales.shape) != (inner // group, columns) or scales.dtype not in (torch.float16, torch.float32):
+            raise ParakeetError(f"{name} scales must be f16 or f32 [{inner // group},{columns}]")
+        if not words.is_cuda or not scales.is_cuda or not scales.is_contiguous() or words.device != scales.device:
+            raise ParakeetError("operands must be contiguous CUDA tensors")
+        nt, kt = -(-columns // 16), -(-inner // 128)
+        w = words.view(torch.int32)
+        if columns % 16 or inner % 128:  # code 8 (weight 0) outside the matrix
+            full = torch.full((nt * 16, kt * 16), -0x77777778, dtype=torch.int32, device=w.device)
+            full[:columns, :inner // 8] = w
+            w = full
+        # [tile row, half, lane / 4, tile column, block of 32 inputs, lane % 4]
+        tiles = w.reshape(nt, 2, 8, kt, 4, 4).permute(0, 3, 1, 2, 5, 4).contiguous().reshape(-1)
+        scalar = "float16" if scales.dtype == torch.float16 else "float32"
+        return Int4Weight(inner, columns, group,
+                          GpuTensor(f"{name}.codes", "uint32", (inner, columns), rp.INT4_TILE_LAYOUT, tiles),
+                          GpuTensor(f"{name}.scales", scalar, (inner // group, columns), rp.INT4_SCALE_LAYOUT, scales))
+
+    @staticmethod
+    def quantize(weight: np.ndarray, group: int, profile: str = "fp16", device: str = "cuda",
+                 name: str = "int4") -> "Int4Weight":
+        """Rounds a host [K, N] weight to 4 bits (rp.quantize_int4)."""
+        _precision(profile)
+        words, scales = rp.quantize_int4(weight, group, profile)
+        return Int4Weight.from_words(torch.from_numpy(words.view(np.int32)).to(device),
+                                     torch.from_numpy(scales).to(device), weight.shape[0], group, name)
+
+
+class Int4GemvKernel:
+    """1 to 64 rows times an Int4Weight (pk_int4_gemv), the decode form of the palette GEMM."""
+
+    MAX_ROWS = 64
+
+    def __init__(self, device: Device, profile: str):
+        self.device, self.profile = device, profile
+
+    @staticmethod
+    def create(device: Device, arena=None, capacity: int = 0, profile: str = "fp16") -> "Int4GemvKernel":
+        _precision(profile)
+        return Int4GemvKernel(device, profile)
+
+    def create_dispatch(self, d: dict) -> _Dispatch:
+        """d: label, a [rows, K], weight (Int4Weight), output [rows, N], rows, activation="none",
+        bias (f32 [N]) or residual [rows, N] with residual_scale=1.0 (residual may be output)."""
+        label, dev, w = d["label"], self.device, d["weight"]
+        (rows,) = _sizes(d, rows=1)
+        if rows > self.MAX_ROWS:
+            raise RangeError(f"{label} rows must be in [1, {self.MAX_ROWS}]")
+        scalar = _scalar_dtype(self.profile)
+        if not isinstance(w, Int4Weight) or w.codes.layout != rp.INT4_TILE_LAYOUT:
+            raise ParakeetError(f"{label} has an unsupported weight format")
+        if w.scales.tensor.dtype != scalar:
+            raise ParakeetError(f"{label} scales must be {scalar}, got {w.scales.tensor.dtype}")
+        if d.get("activation", "none") not in _lib.ACT:
+            raise ParakeetError(f"{label} has an unknown activation {d['activation']!r}")
+        if d.get("bias") is not None and d.get("residual") is not None:
+            raise ParakeetError(f"{label} cannot fuse bias and residual together")
+        if d.get("residual") is None and d.get("residual_scale") is not None:
+            raise ParakeetError(f"{label} supplies a residual scale without a residual")
+        a = _operand(d, "a", scalar, rows * w.inner, dev)
+        out = _operand(d, "output", scalar, rows * w.columns, dev)
+        bias = _operand(d, "bias", torch.float32, w.columns, dev, optional=True)
+        residual = _operand(d, "residual", scalar, rows * w.columns, dev, optional=True)
+        own = {"codes": w.codes, "scales": w.scales, "label": label}
+        codes = _operand(own, "codes", _ids(), -(-w.columns // 16) * -(-w.inner // 128) * 256, dev)
+        scales = _operand(own, "scales", scalar, w.inner // w.group * w.columns, dev)
+        scale = d.get("residual_scale")
+        desc = _lib.Int4GemvDesc(_precision(self.profile), rows, w.inner, w.columns, w.group,
+                                 _lib.ACT[d.get("activation", "none")], 1.0 if scale is None else float(scale),
+                                 *[_address(t) for t in (bias, residual, a, codes, scales, out)])
+        disp = _FixedDispatch(label, dev, "pk_int4_gemv", desc, (bias, residual, a, codes, scales, out))
+        disp.output = d["output"]
+        return disp
+
+
+class JointLogitsKernel:
+    """The joint of the emitted tokens of a batch of windows (pk_joint_logits): ragged rows whose
+    number is known on the device alone, in the form TokenScoresKernel takes."""
+
+    def __init__(self, device: Device, profile: str):
+        self.device, self.profile = device, profile
+
+    @staticmethod
+    def create(device: Device, arena=None, capacity: int = 0, profile: str = "fp16") -> "JointLogitsKernel":
+        _precision(profile)
+        return JointLogitsKernel(device, profile)
+
+    def create_dispatch(self, d: dict) -> _Dispatch:
+        """d: label, encoder_projected [batch, frames, inner], predictor (f32 [batch, max_tokens,
+        inner]), joint_frames (u32 [batch, max_tokens]), counts (u32 [batch]), weight [inner,
+        columns], bias (f32 [columns], optional), logits [batch * max_tokens, columns], row_map
+        (u32 [batch * max_tokens]), row_count (u32 [1]), batch_size, frames, max_tokens, inner,
+        columns."""
+        label, dev = d["label"], self.device
+        b, t, m, inner, columns = _sizes(d, batch_size=1, frames=1, max_tokens=1, inner=1, columns=1)
+        if inner % 32 or columns % 8:
+            raise RangeError(f"Unsupported joint shape for {label}")
+        scalar, f32 = _scalar_dtype(self.profile), torch.float32
+        need = {"encoder_projected": (scalar, b * t * inner), "predictor": (f32, b * m * inner),
+                "joint_frames": (_ids(), b * m), "counts": (_ids(), b), "weight": (scalar, inner * columns),
+                "bias": (f32, columns), "logits": (scalar, b * m * columns), "row_map": (_ids(), b * m),
+                "row_count": (_ids(), 1)}
+        ops = {k: _operand(d, k, dt, n, dev, optional=k == "bias") for k, (dt, n) in need.items()}
+        desc = _lib.JointLogitsDesc(_precision(self.profile), b, t, m, inner, columns,
+                                    *[_address(ops[k]) for k in need])
+        disp = _FixedDispatch(label, dev, "pk_joint_logits", desc, ops)
+        disp.output = d["logits"]
+        return disp
+
+
 def set_gemm_route(route: str) -> None:
     """Test hook: "auto", "simt" (CUDA cores), "tensor" (tcgen05),
     "tensor-single" (tcgen05, single-CTA tiles only) or "tensor-pair"

@@ -28,6 +28,9 @@ TILE_MAJOR_F32_LAYOUT = "n128-k32-tile-major-f32"
 PALETTE5_LAYOUT = "k-by-output-row-major-palette5-lsb-u32"
 PALETTE6_LAYOUT = "k-by-output-row-major-palette6-lsb-u32"
 PALETTE_LUT_LAYOUT = "output-group-by-palette-lut"
+INT4_LAYOUT = "output-by-k-int4-lsb-u32"
+INT4_TILE_LAYOUT = "n16-k128-lane-major-int4-u32"
+INT4_SCALE_LAYOUT = "k-group-by-output-scale"
 TILE_INNER = 32
 
 
@@ -142,3 +145,45 @@ def pack_projected_relative_positions(projected: np.ndarray, heads: int = 8, vec
     head = channels // heads
     return np.ascontiguousarray(
         projected.reshape(p_rows, heads, head // vector_width, vector_width).transpose(1, 2, 0, 3))
+
+
+# --------------------------------------------------------------------- 4-bit weights with group scales
+# No counterpart in the reference, whose packages hold 5- and 6-bit palettes.
+
+def check_int4_geometry(inner: int, columns: int, group: int) -> None:
+    """W[k, n] = (code - 8) * scale[k // group, n]; raises ValueError."""
+    if inner <= 0 or inner % 32 or columns <= 0:
+        raise ValueError(f"int4 weights need K a positive multiple of 32 and N positive, got K={inner}, N={columns}")
+    if group <= 0 or inner % group or (group not in (32, 64) and group % 128):
+        raise ValueError(f"int4 groups are 32, 64 or a multiple of 128 inputs and divide K, got {group} of {inner}")
+
+
+def quantize_int4(weight: np.ndarray, group: int, precision: str = "fp16") -> tuple[np.ndarray, np.ndarray]:
+    """Symmetric 4-bit codes of a [K, N] weight: (words u32 [N, K / 8], scales
+    [K / group, N]).  A group's scale takes its largest magnitude to code 1 or
+    15 (7 steps from the zero code 8); codes are rounded to nearest with the
+    scale as stored."""
+    inner, columns = weight.shape
+    check_int4_geometry(inner, columns, group)
+    w = np.asarray(weight, np.float32).reshape(inner // group, group, columns)
+    scales = (np.abs(w).max(axis=1) / 7.0).astype(np.float16 if precision == "fp16" else np.float32)
+    step = scales.astype(np.float32)[:, None, :]
+    codes = np.rint(np.divide(w, step, out=np.zeros_like(w), where=step > 0)).clip(-8, 7) + 8
+    return pack_int4(codes.reshape(inner, columns).astype(np.uint8)), scales
+
+
+def pack_int4(codes: np.ndarray) -> np.ndarray:
+    """[K, N] codes in 0..15 -> u32 [N, K / 8] (INT4_LAYOUT): eight inputs per word, lowest bits first."""
+    inner, columns = codes.shape
+    if inner % 8:
+        raise ValueError(f"int4 codes need K a multiple of 8, got {inner}")
+    if codes.size and (int(codes.min()) < 0 or int(codes.max()) > 15):
+        raise ValueError("int4 codes must be in [0, 16)")
+    c = np.ascontiguousarray(codes.T).astype(np.uint32).reshape(columns, inner // 8, 8)
+    return np.bitwise_or.reduce(c << np.arange(0, 32, 4, dtype=np.uint32), axis=2).astype("<u4")
+
+
+def unpack_int4(words: np.ndarray) -> np.ndarray:
+    """pack_int4's inverse: u32 [N, K / 8] -> uint8 [K, N]."""
+    c = (words[:, :, None] >> np.arange(0, 32, 4, dtype=np.uint32)) & np.uint32(15)
+    return np.ascontiguousarray(c.reshape(words.shape[0], -1).T).astype(np.uint8)
