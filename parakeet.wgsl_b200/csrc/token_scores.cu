@@ -1,29 +1,38 @@
 // token_scores.cu -- what a row of logits says about a given token: its log
 // probability, the log of the normaliser, the entropy and the best
-// alternatives, in one pass over the row.
+// alternatives, from one read of the row.
 //
 // With m the row's maximum, d_j = x_j - m, s = sum e^{d_j}, u = sum e^{d_j} d_j:
 //   log_sum = m + log s,  log_prob(t) = d_t - log s,  entropy = log s - u / s,
-// and the K best (value, then lower index) with their d - log s.  A thread
-// keeps a running (m, s, u): when its maximum grows by g, s becomes s e^{-g}
-// and u becomes (u - g s) e^{-g}.  Statistics are f32 whatever the logits' type
-// and use x - m itself (exact near the maximum), not x log2(e) - m log2(e).
-// A masked (-inf) logit has d clamped to -200, where e^d is zero, so that it
-// adds 0 to u and not 0 * -inf; the clamp passes NaN on.  A row with a NaN or a
-// +inf has no distribution: its numbers are NaN, its alternatives still rank
-// (NaN as -inf).  A row of -inf alone scores -inf with entropy 0.
+// and the K best (value, then lower index) with their d - log s.  The sums run
+// in base 2: t_j = x_j L - b with L = log2(e) as rounded and b = m L rounded is
+// one FMA, and exact up to its own rounding; b's rounding r = m L - b shifts
+// every t alike and is taken out at the end.  Parts of a row with bases b and
+// b + g join as s 2^{-g}, (u - g s) 2^{-g}.  Statistics are f32 whatever the
+// logits' type.  A masked (-inf) logit has t clamped, to where 2^t is zero, so
+// that it adds 0 to u and not 0 * -inf; the clamp passes NaN on.  A row with a
+// NaN or a +inf has no distribution: its numbers are NaN, its alternatives
+// still rank (NaN as -inf).  A row of -inf alone scores -inf with entropy 0.
 //
-// Alternatives: a warp keeps its K best in registers, lane i the i-th, and
-// inserts a candidate with one ballot and two shuffles.  Few values get that
-// far: a tile is looked at only if some lane's maximum reaches the K-th best
-// value any warp of the row has seen (one shared word, only ever raised), and
-// the first tile starts from the K-th largest of the warp's 32 lane maxima.
-// Joining lists counts, for every entry, how many entries beat it: its rank.
+// Two routes.  HELD: the warps of a row hold it in registers, so the maximum
+// is known before the first exponential.  STREAM: longer rows pass through
+// once with a running (m, s, u) per thread.
 //
-// Bound by reading the logits once.  A row is read by one warp, several warps
-// of a CTA or a cluster of CTAs (joined through distributed shared memory: no
-// workspace, no atomics on results, so results do not depend on timing).
+// Alternatives cost nothing while the row is read: a lane knows its largest
+// value, and lane maxima bound the K-th best value from below: where every one
+// of the row's w warps has ceil(K / w) lanes that reach a value, K columns do.
+// Few values reach that bound (about K times the w-th harmonic number); they
+// go to a pool in shared memory and each counts how many of the pool beat it:
+// its rank.  A pool that
+// overflows (a row of many equal values) is replaced by sorted lists, one per
+// warp, into which candidates are inserted one at a time.  Where fewer than K
+// columns are left by a mask, the lowest masked ids fill the places.
+//
+// Bound by reading the logits once.  A row belongs to one warp, to several
+// warps of a CTA or to a cluster of CTAs (joined through distributed shared
+// memory: no workspace, no atomics, so results do not depend on timing).
 #include <algorithm>
+#include <climits>
 
 #include "pk_common.cuh"
 #include "pk_internal.h"
@@ -34,9 +43,14 @@ namespace {
 constexpr int TS_WARPS = 8;              // warps per CTA
 constexpr int TS_THREADS = TS_WARPS * 32;
 constexpr int TS_MAXK = 32;              // one alternative per lane
-constexpr int TS_UNR = 4;                // 16-byte vectors per lane and tile
 constexpr int TS_CLUSTER = 8;            // CTAs that share a row, at most
+constexpr int TS_HELD = 10;              // 16-byte vectors per lane of a held row, at most
+constexpr int TS_HELD_FEW = 4;           // and where there are few rows: more warps, shorter chains
+constexpr int TS_UNR = 4;                // vectors per lane and tile of a streamed row
+constexpr int TS_POOL = 128;             // candidates per warp of a row
+constexpr uint32_t TS_MASKED = 0x007fffffu;  // ts_ordered(-inf)
 constexpr float TS_LOG2E = 1.4426950408889634f;
+constexpr float TS_LN2 = 0.6931471805599453f;
 
 struct TsParams {
   const void* logits;
@@ -52,19 +66,21 @@ struct TsParams {
   int columns, k;
 };
 
+// A part of a row: its maximum, and the sums in base 2 relative to ts_base(m).
 struct TsStat {
   float m, s, u;
 };
 
 struct TsSmem {
-  alignas(16) unsigned char stage[TS_WARPS][32 * 16];  // one lane's tile, or the warp's lane maxima
-  float lv[TS_WARPS][TS_MAXK];                         // the warps' lists
-  uint32_t li[TS_WARPS][TS_MAXK];
-  float cv[TS_CLUSTER][TS_MAXK];                       // the cluster's lists (rank 0 holds them all)
-  uint32_t ci[TS_CLUSTER][TS_MAXK];
+  alignas(16) unsigned char stage[TS_WARPS][TS_HELD * 16];  // one lane's values
+  uint64_t pool[TS_WARPS * TS_POOL];     // candidates: TS_POOL places per warp of the row (or its sorted lists)
+  uint64_t final[TS_WARPS][TS_MAXK];     // per row: the K best, in order
+  uint64_t clist[TS_CLUSTER][TS_MAXK];   // the K best of the cluster's CTAs (rank 0 holds them all)
   TsStat stat[TS_WARPS];
   TsStat cstat[TS_CLUSTER];
-  uint32_t bound[TS_WARPS];                            // per row of the CTA: ordered bits of the K-th best value seen
+  alignas(16) uint32_t lane_max[TS_WARPS][32];
+  uint32_t bound[TS_WARPS];              // per warp
+  int count[TS_WARPS];                   // per row: candidates
 };
 
 __device__ __forceinline__ float ts_ex2(float x) {
@@ -77,197 +93,256 @@ __device__ __forceinline__ float ts_max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
-// Order-preserving bits of a float (its own zero: -0 counts as 0).
+// Order-preserving bits of a float (its own zero: -0 counts as 0), and back.
 __device__ __forceinline__ uint32_t ts_ordered(float v) {
   const uint32_t b = __float_as_uint(v + 0.0f);
   return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
-__device__ __forceinline__ bool ts_beats(float av, uint32_t ai, float bv, uint32_t bi) {
-  return av > bv || (av == bv && ai < bi);
+__device__ __forceinline__ float ts_value(uint32_t o) {
+  return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
+}
+// A place in the order of alternatives: larger is better.  0 is an empty place.
+__device__ __forceinline__ uint64_t ts_key(float v, uint32_t id) {
+  return (uint64_t)ts_ordered(v != v ? -INFINITY : v) << 32 | (uint32_t)~id;
 }
 
-// (m, s, u) of two parts of a row.
+// The factor of x in t (beyond 1e37, where x L could overflow, neighbouring
+// values are so far apart that any factor gives 2^t = 0 or 1) and the base.
+__device__ __forceinline__ float ts_factor(float m) { return fabsf(m) <= 1e37f ? TS_LOG2E : 1.0f; }
+__device__ __forceinline__ float ts_base(float m) { return m > -INFINITY ? __fmul_rn(m, ts_factor(m)) : 0.0f; }
+
+// (s, u) of base b rescaled to a base that is larger by -g.
+__device__ __forceinline__ void ts_shift(float g, float& s, float& u) {
+  const float c = ts_ex2(g);
+  u = c == 0.0f ? 0.0f : c * fmaf(g, s, u);  // once 2^g is 0 nothing is left
+  s *= c;
+}
 __device__ __forceinline__ TsStat ts_join(TsStat a, TsStat b) {
-  const float m = fmaxf(a.m, b.m);
-  TsStat r{m, 0.0f, 0.0f};
-  auto add = [&](const TsStat& p) {
+  TsStat r{fmaxf(a.m, b.m), 0.0f, 0.0f};
+  auto add = [&](TsStat p) {
     if (p.s == 0.0f) return;  // nothing but masked logits
-    const float g = p.m == m ? 0.0f : p.m - m;
-    const float c = ts_ex2(g * TS_LOG2E);
-    r.s = fmaf(p.s, c, r.s);
-    // The part's share after rescaling; e^g g is 0 once e^g is.
-    r.u = fmaf(c, c > 0.0f || c != c ? fmaf(g, p.s, p.u) : 0.0f, r.u);
+    if (p.m != r.m) ts_shift(ts_base(p.m) - ts_base(r.m), p.s, p.u);
+    r.s += p.s;
+    r.u += p.u;
   };
   add(a);
   add(b);
   return r;
 }
 
-template <typename T>
+// The sums of the `n` (at most 8) parts of a row, in their order.
+__device__ __forceinline__ TsStat ts_join_warps(const TsStat* part, int n) {
+  TsStat st = part[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i)
+    if (i < n) st = ts_join(st, part[i]);
+  return st;
+}
+
+// N 16-byte vectors of a row per lane.
+template <typename T, int N>
 struct TsTile {
   static constexpr int VEC = 16 / sizeof(T);
   static constexpr uint32_t NEG = sizeof(T) == 2 ? 0xfc00fc00u : 0xff800000u;  // -inf
-  uint4 raw[TS_UNR];
+  uint4 raw[N];
 
-  // Vectors v0, v0 + 32, ... of the row, which starts `skew` elements into its
-  // first 16-byte vector; a vector that is not whole is read element by element.
-  __device__ __forceinline__ void load(const T* base, int skew, int columns, int v0, int vectors) {
+  // Vector v of a row that starts `skew` elements into its first 16 bytes; what
+  // is not of the row reads as -inf, and is not read.
+  static __device__ __forceinline__ uint4 vector(const T* base, int skew, int columns, int v, int vectors) {
+    const int c0 = v * VEC - skew;
+    uint4 r = make_uint4(NEG, NEG, NEG, NEG);
+    if (v < vectors) {
+      if (c0 >= 0 && c0 + VEC <= columns) {
+        r = __ldcs(reinterpret_cast<const uint4*>(base + c0));
+      } else {
+        T* e = reinterpret_cast<T*>(&r);
 #pragma unroll
-    for (int q = 0; q < TS_UNR; ++q) {
-      const int v = v0 + 32 * q;
-      const int c0 = v * VEC - skew;
-      raw[q] = make_uint4(NEG, NEG, NEG, NEG);
-      if (v < vectors) {
-        if (c0 >= 0 && c0 + VEC <= columns) {
-          raw[q] = __ldcs(reinterpret_cast<const uint4*>(base + c0));
-        } else {
-          T* e = reinterpret_cast<T*>(&raw[q]);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            if (c0 + j >= 0 && c0 + j < columns) e[j] = base[c0 + j];
-        }
+        for (int j = 0; j < VEC; ++j)
+          if (c0 + j >= 0 && c0 + j < columns) e[j] = base[c0 + j];
       }
     }
+    return r;
   }
-  __device__ __forceinline__ float maximum() const {
+  // Vectors v0 + lane + step q; `v0` is the warp's.
+  __device__ __forceinline__ void load(const T* base, int skew, int columns, int v0, int lane, int step, int vectors) {
+    if (v0 * VEC >= skew && (v0 + step * (N - 1) + 32) * VEC - skew <= columns) {  // all of them whole
+      const uint4* src = reinterpret_cast<const uint4*>(base + (v0 + lane) * VEC - skew);
+#pragma unroll
+      for (int q = 0; q < N; ++q) raw[q] = __ldcs(src + step * q);
+    } else {
+#pragma unroll
+      for (int q = 0; q < N; ++q) raw[q] = vector(base, skew, columns, v0 + lane + step * q, vectors);
+    }
+  }
+  static __device__ __forceinline__ float largest(const uint4* raw, int n) {
     if constexpr (sizeof(T) == 2) {
       __half2 mx = *reinterpret_cast<const __half2*>(&raw[0].x);
 #pragma unroll
-      for (int q = 0; q < TS_UNR; ++q) {
+      for (int q = 0; q < n; ++q) {
         const __half2* h = reinterpret_cast<const __half2*>(&raw[q]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) mx = __hmax2(mx, h[j]);
       }
       const float2 f = __half22float2(mx);
-      return fmaxf(fmaxf(f.x, f.y), -INFINITY);
+      return fmaxf(fmaxf(f.x, f.y), -INFINITY);  // NaN counts as -inf
     } else {
       float mx = -INFINITY;
 #pragma unroll
-      for (int q = 0; q < TS_UNR; ++q) {
+      for (int q = 0; q < n; ++q) {
         const float* f = reinterpret_cast<const float*>(&raw[q]);
         mx = fmaxf(mx, fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])));
       }
       return mx;
     }
   }
-  template <typename F>
-  __device__ __forceinline__ void pairs(F f) const {
+  __device__ __forceinline__ float maximum() const { return largest(raw, N); }
+  // s += sum 2^t, u += sum 2^t t for t = x ts_factor(m) - ts_base(m).
+  __device__ __forceinline__ void sums(float m, float2& s, float2& u) const {
+    const float a = ts_factor(m), b = -ts_base(m);
+    const float2 a2 = make_float2(a, a), b2 = make_float2(b, b), one = make_float2(1.0f, 1.0f);
+    auto add = [&](float2 t) {
+      const float2 e = make_float2(ts_ex2(t.x), ts_ex2(t.y));
+      s = ffma2(e, one, s);
+      u = ffma2(e, t, u);
+    };
+    if constexpr (sizeof(T) == 2) {
+      // -inf becomes the lowest f16 before the conversion, two at a time: for
+      // any m above it by 300 or more that is a 2^t of 0.
+      if (m > -60000.0f) {
+        const __half2 low = __float2half2_rn(-65504.0f);
 #pragma unroll
-    for (int q = 0; q < TS_UNR; ++q) {
+        for (int q = 0; q < N; ++q) {
+          const __half2* h = reinterpret_cast<const __half2*>(&raw[q]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) add(ffma2(__half22float2(__hmax2_nan(h[j], low)), a2, b2));
+        }
+        return;
+      }
+    }
+    auto clamped = [&](float2 x) {
+      float2 t = ffma2(x, a2, b2);
+      t.x = ts_max_nan(t.x, -300.0f);
+      t.y = ts_max_nan(t.y, -300.0f);
+      add(t);
+    };
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
       if constexpr (sizeof(T) == 2) {
         const __half2* h = reinterpret_cast<const __half2*>(&raw[q]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f(__half22float2(h[j]));
+        for (int j = 0; j < 4; ++j) clamped(__half22float2(h[j]));
       } else {
         const float2* h = reinterpret_cast<const float2*>(&raw[q]);
-        f(h[0]);
-        f(h[1]);
+        clamped(h[0]);
+        clamped(h[1]);
       }
     }
   }
 };
 
-// A warp's K best: lane i holds the i-th (value, index); an empty place is
-// (-inf, ~0).
-struct TsList {
-  float v = -INFINITY;
-  uint32_t i = 0xffffffffu;
-
-  // Inserts (cv, ci), the same in all lanes.
-  __device__ __forceinline__ void insert(float cv, uint32_t ci, int k, int lane) {
-    const int pos = __popc(__ballot_sync(0xffffffffu, ts_beats(v, i, cv, ci)));
-    const float pv = __shfl_up_sync(0xffffffffu, v, 1);
-    const uint32_t pi = __shfl_up_sync(0xffffffffu, i, 1);
-    if (pos >= k) return;
-    if (lane == pos) {
-      v = cv;
-      i = ci;
-    } else if (lane > pos) {
-      v = pv;
-      i = pi;
-    }
-  }
-};
-
-// Looks at the tile's lanes whose maximum reaches `bound`: each such lane's
-// values are spread over the warp through `stage`, and those that reach the
-// bound are inserted.  Returns the raised bound.
-template <typename T>
-__device__ __forceinline__ uint32_t ts_candidates(const TsTile<T>& tile, TsList& list, unsigned char* stage, uint32_t mine,
-                                               uint32_t bound, int v0, int skew, int columns, int k, int lane) {
-  constexpr int VEC = TsTile<T>::VEC;
-  constexpr int EPL = VEC * TS_UNR;
-  uint32_t lanes = __ballot_sync(0xffffffffu, mine >= bound);
-  while (lanes) {
-    const int src = __ffs(lanes) - 1;
-    lanes &= lanes - 1;
-    if (__shfl_sync(0xffffffffu, mine, src) < bound) continue;  // the bound rose meanwhile
-    __syncwarp();
-    if (lane == src) {
-#pragma unroll
-      for (int q = 0; q < TS_UNR; ++q) reinterpret_cast<uint4*>(stage)[q] = tile.raw[q];
-    }
-    __syncwarp();
-    float v = -INFINITY;
-    uint32_t id = 0xffffffffu;
-    if (lane < EPL) {
-      v = (float)reinterpret_cast<const T*>(stage)[lane];
-      if (v != v) v = -INFINITY;
-      const int c = (v0 - lane + src + 32 * (lane / VEC)) * VEC - skew + lane % VEC;
-      if (c >= 0 && c < columns) id = (uint32_t)c;
-    }
-    uint32_t cand = __ballot_sync(0xffffffffu, id != 0xffffffffu && ts_ordered(v) >= bound);
-    while (cand) {
-      const int from = __ffs(cand) - 1;
-      cand &= cand - 1;
-      list.insert(__shfl_sync(0xffffffffu, v, from), __shfl_sync(0xffffffffu, id, from), k, lane);
-    }
-    // The K-th best so far, once there are K.
-    const uint32_t last = __shfl_sync(0xffffffffu, list.i, k - 1);
-    if (last != 0xffffffffu) bound = max(bound, ts_ordered(__shfl_sync(0xffffffffu, list.v, k - 1)));
-  }
-  return bound;
+// Inserts `key`, the same in all lanes, into the list (lane i holds the i-th).
+__device__ __forceinline__ void ts_insert(uint64_t& list, uint64_t key, int lane) {
+  const int pos = __popc(__ballot_sync(0xffffffffu, list > key));
+  const uint64_t prev = __shfl_up_sync(0xffffffffu, list, 1);
+  if (lane == pos) list = key;
+  else if (lane > pos) list = prev;
 }
 
-// Ranks `n` entries (value, index; ties of empty places by position) and hands
-// each of the best `k` to out(rank, value, index).
-template <typename Out>
-__device__ __forceinline__ void ts_rank(const float* v, const uint32_t* id, int lists, int k, int t, int threads, Out out) {
-  const int n = lists * k;
-  for (int e = t; e < n; e += threads) {
-    const float ev = v[e / k * TS_MAXK + e % k];
-    const uint32_t ei = id[e / k * TS_MAXK + e % k];
-    int rank = e % k;  // a list is in order
-    for (int l = 0; l < lists; ++l) {
-      if (l == e / k) continue;
-      for (int j = 0; j < k; ++j) {
-        const float ov = v[l * TS_MAXK + j];
-        const uint32_t oi = id[l * TS_MAXK + j];
-        // Equal entries are empty places: the earlier list's come first.
-        const bool beats = ts_beats(ov, oi, ev, ei) || (ov == ev && oi == ei && l < e / k);
-        if (!beats) break;
-        ++rank;
-      }
-    }
-    if (rank < k) out(rank, ev, ei);
+// Inserts those of the lanes' keys that beat the list's K-th (each lane offers
+// one; 0 offers nothing).
+__device__ __forceinline__ void ts_offer(uint64_t& list, uint64_t key, int k, int lane) {
+  uint64_t last = __shfl_sync(0xffffffffu, list, k - 1);
+  uint32_t lanes = __ballot_sync(0xffffffffu, key > last);
+  while (lanes) {
+    const int src = __ffs(lanes) - 1;
+    const uint64_t c = __shfl_sync(0xffffffffu, key, src);
+    ts_insert(list, c, lane);
+    last = __shfl_sync(0xffffffffu, list, k - 1);
+    if (lane == src) key = 0;
+    lanes = __ballot_sync(0xffffffffu, key > last);
   }
+}
+
+// How many entries of the `lists` sorted lists (k entries each, `pitch` apart)
+// come before entry `pos` of list `own`; equal entries in order of their lists.
+template <typename U>
+__device__ __forceinline__ int ts_rank(const U* list, int pitch, int lists, int k, int own, int pos) {
+  const U key = list[own * pitch + pos];
+  int rank = pos;
+#pragma unroll
+  for (int l = 0; l < 8; ++l) {
+    if (l >= lists || l == own) continue;
+    const U* other = list + l * pitch;
+    int n = 0;
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1) {
+      const int i = n + step;
+      if (i <= k && (other[i - 1] > key || (other[i - 1] == key && l < own))) n = i;
+    }
+    rank += n;
+  }
+  return rank;
+}
+
+// Barrier of the `wpr` warps of a row (barrier 0 is the CTA's).
+__device__ __forceinline__ void ts_row_sync(int group, int wpr) {
+  if (wpr == 1) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(wpr * 32) : "memory");
+}
+
+// A value (ordered bits) that at least k of the row's columns in this CTA
+// reach, where k are unmasked: the least of the warps' j-th largest lane
+// maxima, j = ceil(k / wpr).  More than -inf: no masked value is a candidate.
+__device__ __forceinline__ uint32_t ts_bound(TsSmem& sm, uint32_t mine, int group, int wpr, int k) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int j = (k + wpr - 1) / wpr;
+  uint32_t bound;
+  if (j == 1) {
+    bound = __reduce_max_sync(0xffffffffu, mine);
+  } else {
+    sm.lane_max[warp][lane] = mine;
+    __syncwarp();
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint4 o = reinterpret_cast<const uint4*>(sm.lane_max[warp])[i];
+      above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+    }
+    bound = __reduce_min_sync(0xffffffffu, above < j ? mine : 0xffffffffu);
+  }
+  if (wpr > 1) {
+    if (lane == 0) sm.bound[warp] = bound;
+    ts_row_sync(group, wpr);
+    bound = sm.bound[group * wpr];
+#pragma unroll
+    for (int w = 1; w < 8; ++w)
+      if (w < wpr) bound = min(bound, sm.bound[group * wpr + w]);
+  }
+  return max(bound, TS_MASKED + 1);
+}
+
+// Whether the row's candidates did not fit the pool.
+__device__ __forceinline__ bool ts_overflow(TsSmem& sm, int group, int wpr) {
+  ts_row_sync(group, wpr);
+  return sm.count[group] > wpr * TS_POOL;
 }
 
 // `wpr` warps of the CTA read one row (8 / wpr rows per CTA); with CLUSTER the
-// CTAs of a cluster share one row.
-template <typename T, bool CLUSTER>
-__global__ void __launch_bounds__(TS_THREADS) token_scores_kernel(const TsParams p, int wpr) {
+// CTAs of a cluster share one row.  NV: vectors per lane of a held row, 0: the
+// row is streamed.
+template <typename T, int NV, bool CLUSTER>
+__global__ void __launch_bounds__(TS_THREADS, sizeof(T) == 2 && NV > 0 ? (NV == TS_HELD ? 2 : 3) : NV == TS_HELD ? 3 : 4) token_scores_kernel(const TsParams p, int wpr) {
   pdl_entry();
   // Distributed shared memory is written only after this barrier's wait: by
   // then every CTA of the cluster runs.
   if constexpr (CLUSTER) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   __shared__ TsSmem sm;
+  constexpr int VEC = 16 / sizeof(T);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int group = warp / wpr, wig = warp % wpr;  // row of the CTA, warp of the row
   const int ranks = CLUSTER ? (int)gridDim.x : 1;  // the grid is (cluster, rows) then
   const int rank = CLUSTER ? (int)blockIdx.x : 0;
-  const int64_t row = CLUSTER ? (int64_t)blockIdx.y + (int64_t)blockIdx.z * gridDim.y
-                              : (int64_t)blockIdx.x * (TS_WARPS / wpr) + group;
+  const int64_t row = CLUSTER ? (int64_t)blockIdx.y : (int64_t)blockIdx.x * (TS_WARPS / wpr) + group;
   const int64_t rows = p.row_count ? min(p.rows, (int64_t)*p.row_count) : p.rows;
   int64_t slot = row;
   bool live = row < rows;
@@ -277,77 +352,104 @@ __global__ void __launch_bounds__(TS_THREADS) token_scores_kernel(const TsParams
   }
   const int k = p.k;
   const T* base = static_cast<const T*>(p.logits) + (live ? row : 0) * p.stride;
-  uint32_t target = 0;
   float given = -INFINITY;
   if (live && p.targets && wig == 0 && lane == 0 && rank == 0) {
-    target = p.targets[slot];
+    const uint32_t target = p.targets[slot];
     given = target < (uint32_t)p.columns ? (float)base[target] : NAN;  // an id outside the row has no probability
   }
-  if (tid < TS_WARPS) sm.bound[tid] = 0;
+  const int skew = (int)((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
+  const int vectors = live ? (int)(((int64_t)skew + p.columns + VEC - 1) / VEC) : 0;
+  const int columns = p.columns;
+  const int warps = wpr * ranks, gw = rank * wpr + wig;  // warps of the row, this one
+  unsigned char* stage = sm.stage[warp];
+  uint64_t list = 0;
+  bool overflow = false;
+  TsStat st;
+  if (tid < TS_WARPS) sm.count[tid] = 0;
   __syncthreads();
+  auto offer = [&](float v, int id) {
+    const int at = atomicAdd(&sm.count[group], 1);
+    if (at < wpr * TS_POOL) sm.pool[group * wpr * TS_POOL + at] = ts_key(v, (uint32_t)id);
+  };
 
-  TsList list;
-  TsStat st{-INFINITY, 0.0f, 0.0f};
-  if (live) {
-    const int skew = (int)((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
-    const int vectors = (int)(((int64_t)skew + p.columns + TsTile<T>::VEC - 1) / TsTile<T>::VEC);
-    const int step = wpr * ranks * 32 * TS_UNR;
-    int v0 = (rank * wpr + wig) * 32 * TS_UNR + lane;
+  if constexpr (NV > 0) {
+    // Vector q of a lane: (q * warps + gw) * 32 + lane.
+    const int step = warps * 32, v0 = gw * 32 + lane;
+    TsTile<T, NV> tile;
+    tile.load(base, skew, columns, gw * 32, lane, step, vectors);
+    const float mine = tile.maximum();
+    st.m = ts_value(__reduce_max_sync(0xffffffffu, ts_ordered(mine)));
+    float2 s2 = make_float2(0.0f, 0.0f), u2 = make_float2(0.0f, 0.0f);
+    tile.sums(st.m, s2, u2);
+    st.s = s2.x + s2.y;
+    st.u = u2.x + u2.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
+      st.u += __shfl_xor_sync(0xffffffffu, st.u, o);
+    }
+    if (k > 0) {
+      const float bound = ts_value(ts_bound(sm, ts_ordered(mine), group, wpr, k));
+#pragma unroll
+      for (int q = 0; q < NV; ++q) {
+        if (TsTile<T, 1>::largest(&tile.raw[q], 1) >= bound) {
+          const T* e = reinterpret_cast<const T*>(&tile.raw[q]);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            if ((float)e[j] >= bound) offer((float)e[j], (v0 + step * q) * VEC - skew + j);
+        }
+      }
+      if (ts_overflow(sm, group, wpr)) {
+        uint32_t lanes = __ballot_sync(0xffffffffu, mine >= bound);
+        while (lanes) {
+          const int src = __ffs(lanes) - 1;
+          lanes &= lanes - 1;
+          __syncwarp();
+          if (lane == src) {
+#pragma unroll
+            for (int q = 0; q < NV; ++q) reinterpret_cast<uint4*>(stage)[q] = tile.raw[q];
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i0 = 0; i0 < NV * VEC; i0 += 32) {
+            const int i = i0 + lane;
+            uint64_t c = 0;
+            if (i < NV * VEC) {
+              const float v = (float)reinterpret_cast<const T*>(stage)[i];
+              const int id = (v0 - lane + src + step * (i / VEC)) * VEC - skew + i % VEC;
+              if (v >= bound) c = ts_key(v, (uint32_t)id);
+            }
+            ts_offer(list, c, k, lane);
+          }
+        }
+        overflow = true;
+      }
+    }
+  } else {
+    const int step = warps * 32 * TS_UNR, first = gw * 32 * TS_UNR;
     float2 s2 = make_float2(0.0f, 0.0f), u2 = make_float2(0.0f, 0.0f);
     float m = -INFINITY;
-    TsTile<T> tile, next;
-    const int first = v0 - lane;
-    tile.load(base, skew, p.columns, v0, vectors);
-    for (; v0 - lane < vectors; v0 += step) {
-      if (v0 - lane + step < vectors) next.load(base, skew, p.columns, v0 + step, vectors);
+    auto take = [&](const TsTile<T, TS_UNR>& tile) {
       const float tm = tile.maximum();
       if (tm > m) {
         if (m > -INFINITY) {
-          const float g = m - tm;
-          const float c = ts_ex2(g * TS_LOG2E);
-          // Once e^g is 0 nothing of the old sums is left.
-          u2.x = c > 0.0f ? fmaf(g, s2.x, u2.x) * c : 0.0f;
-          u2.y = c > 0.0f ? fmaf(g, s2.y, u2.y) * c : 0.0f;
-          s2.x *= c;
-          s2.y *= c;
+          const float g = ts_base(m) - ts_base(tm);
+          ts_shift(g, s2.x, u2.x);
+          ts_shift(g, s2.y, u2.y);
         }
         m = tm;
       }
-      const float neg = m > -INFINITY ? -m : 0.0f;
-      tile.pairs([&](float2 x) {
-        float2 d = ffma2(x, make_float2(1.0f, 1.0f), make_float2(neg, neg));
-        d.x = ts_max_nan(d.x, -200.0f);
-        d.y = ts_max_nan(d.y, -200.0f);
-        const float2 t = ffma2(d, make_float2(TS_LOG2E, TS_LOG2E), make_float2(0.0f, 0.0f));
-        const float2 e = make_float2(ts_ex2(t.x), ts_ex2(t.y));
-        s2 = ffma2(e, make_float2(1.0f, 1.0f), s2);
-        u2 = ffma2(e, d, u2);
-      });
-      if (k > 0) {
-        const uint32_t mine = ts_ordered(tm);
-        uint32_t bound = *(volatile uint32_t*)&sm.bound[group];
-        if (v0 - lane == first) {
-          // The K-th largest lane maximum: K values of the tile reach it.
-          float* mx = reinterpret_cast<float*>(sm.stage[warp]);
-          mx[lane] = tm;
-          __syncwarp();
-          int above = 0;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float4 o = reinterpret_cast<const float4*>(mx)[j];
-            above += (o.x > tm) + (o.y > tm) + (o.z > tm) + (o.w > tm);
-          }
-          bound = max(bound, __reduce_min_sync(0xffffffffu, above < k ? mine : 0xffffffffu));
-          __syncwarp();
-        }
-        if (__any_sync(0xffffffffu, mine >= bound)) {
-          const uint32_t raised =
-              ts_candidates<T>(tile, list, sm.stage[warp], mine, bound, v0, skew, p.columns, k, lane);
-          if (lane == 0) atomicMax(&sm.bound[group], raised);
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < TS_UNR; ++q) tile.raw[q] = next.raw[q];
+      tile.sums(m, s2, u2);
+    };
+    // The next tile is on its way while one is summed.
+    TsTile<T, TS_UNR> a, b;
+    if (first < vectors) a.load(base, skew, columns, first, lane, 32, vectors);
+    for (int v = first; v < vectors; v += 2 * step) {
+      if (v + step < vectors) b.load(base, skew, columns, v + step, lane, 32, vectors);
+      take(a);
+      if (v + step >= vectors) break;
+      if (v + 2 * step < vectors) a.load(base, skew, columns, v + 2 * step, lane, 32, vectors);
+      take(b);
     }
     st = TsStat{m, s2.x + s2.y, u2.x + u2.y};
 #pragma unroll
@@ -357,65 +459,128 @@ __global__ void __launch_bounds__(TS_THREADS) token_scores_kernel(const TsParams
       // Both lanes of a pair join in the same order.
       st = (lane & o) ? ts_join(other, st) : ts_join(st, other);
     }
+    if (k > 0) {
+      const float bound = ts_value(ts_bound(sm, ts_ordered(m), group, wpr, k));
+      // A lane that reaches it: its vectors, read again, 32 at a time.
+      const uint32_t reach = __ballot_sync(0xffffffffu, m >= bound);
+      const int own = first < vectors ? (vectors - first + step - 1) / step * TS_UNR : 0;
+      auto again = [&](auto use) {
+        for (uint32_t lanes = reach; lanes; lanes &= lanes - 1) {
+          const int src = __ffs(lanes) - 1;
+          for (int i0 = 0; i0 < own; i0 += 32) {
+            const int i = i0 + lane;
+            const int v = i < own ? first + i / TS_UNR * step + 32 * (i % TS_UNR) + src : vectors;
+            use(TsTile<T, 1>::vector(base, skew, columns, v, vectors), v * VEC - skew);
+          }
+        }
+      };
+      again([&](const uint4& raw, int c0) {
+        if (TsTile<T, 1>::largest(&raw, 1) >= bound) {
+          const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            if ((float)e[j] >= bound) offer((float)e[j], c0 + j);
+        }
+      });
+      if (ts_overflow(sm, group, wpr)) {
+        again([&](const uint4& raw, int c0) {
+          const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            ts_offer(list, (float)e[j] >= bound ? ts_key((float)e[j], (uint32_t)(c0 + j)) : 0, k, lane);
+        });
+        overflow = true;
+      }
+    }
   }
-  if (lane == 0) sm.stat[warp] = st;
-  sm.lv[warp][lane] = list.v;
-  sm.li[warp][lane] = list.i;
-  __syncthreads();
-  // Every thread of the row joins the warps' sums (the same numbers in all).
-  st = sm.stat[group * wpr];
-  for (int w = 1; w < wpr; ++w) st = ts_join(st, sm.stat[group * wpr + w]);
-  const float* lv = sm.lv[group * wpr];
-  const uint32_t* li = sm.li[group * wpr];
-  int lists = wpr;
-  if constexpr (CLUSTER) {
-    // This CTA's list and sums go to the first CTA's shared memory.
+  if (CLUSTER || wpr > 1) {
+    if (lane == 0) sm.stat[warp] = st;
+  }
+  if (k > 0) {
+    // This CTA's K best, in order, to `final` (or the first CTA's clist).
+    auto put = [&](int place, uint64_t key) {
+      if (place >= k) return;
+      if constexpr (CLUSTER) {
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_shared(smem_addr(&sm.clist[rank][place]), 0)), "l"(key)
+                     : "memory");
+      } else {
+        sm.final[group][place] = key;
+      }
+    };
+    if constexpr (CLUSTER) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (overflow) {
+      ts_row_sync(group, wpr);
+      uint64_t* lists = sm.pool + group * wpr * TS_POOL;
+      if (lane < k) lists[wig * TS_MAXK + lane] = list;
+      ts_row_sync(group, wpr);
+      if (lane < k) put(ts_rank(lists, TS_MAXK, wpr, k, wig, lane), list);
+    } else {
+      const int n = sm.count[group];
+      const uint64_t* pool = sm.pool + group * wpr * TS_POOL;
+      for (int i = wig * 32 + lane; i < n; i += wpr * 32) {
+        const uint64_t key = pool[i];
+        int place = 0;
+        for (int j = 0; j < n; ++j) place += pool[j] > key ? 1 : 0;
+        put(place, key);
+      }
+      for (int i = n + wig * 32 + lane; i < k; i += wpr * 32) put(i, 0);
+    }
+  } else if constexpr (CLUSTER) {
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    const uint32_t cv = mapa_shared(smem_addr(&sm.cv[rank][0]), 0), ci = mapa_shared(smem_addr(&sm.ci[rank][0]), 0);
-    ts_rank(lv, li, lists, k, tid, TS_THREADS, [&](int r, float v, uint32_t id) {
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cv + 4 * r), "f"(v) : "memory");
-      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(ci + 4 * r), "r"(id) : "memory");
-    });
+  }
+  if constexpr (CLUSTER) {
+    __syncthreads();  // the warps' sums
     if (tid == 0) {
+      st = ts_join_warps(sm.stat, TS_WARPS);
       const uint32_t cs = mapa_shared(smem_addr(&sm.cstat[rank]), 0);
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cs), "f"(st.m) : "memory");
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cs + 4), "f"(st.s) : "memory");
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cs + 8), "f"(st.u) : "memory");
     }
-    __syncthreads();
+    __syncwarp();
     cluster_sync();
     if (rank != 0) return;
-    st = sm.cstat[0];
-    for (int r = 1; r < ranks; ++r) st = ts_join(st, sm.cstat[r]);
-    lv = sm.cv[0];
-    li = sm.ci[0];
-    lists = ranks;
+    if (lane < k && warp < ranks) {
+      const uint64_t key = sm.clist[warp][lane];
+      const int place = ts_rank(&sm.clist[0][0], TS_MAXK, ranks, k, warp, lane);
+      if (place < k) sm.final[0][place] = key;
+    }
   }
-  if (!live) return;
+  if (k > 0 || wpr > 1) ts_row_sync(group, wpr);
+  if (!live || wig != 0) return;
+  if constexpr (CLUSTER) st = ts_join_warps(sm.cstat, ranks);
+  else if (wpr > 1) st = ts_join_warps(sm.stat + group * wpr, wpr);
   const bool empty = st.s == 0.0f;
-  const float log_s = empty ? 0.0f : logf(st.s);
-  if (wig == 0 && lane == 0) {
+  const float r = fmaf(st.m, ts_factor(st.m), -ts_base(st.m)) * TS_LN2;  // the base's rounding
+  const float log_s = empty ? 0.0f : logf(st.s) - r;
+  if (lane == 0) {
     if (p.log_probs) p.log_probs[slot] = empty ? (given == given ? -INFINITY : NAN) : (given - st.m) - log_s;
     if (p.log_sums) p.log_sums[slot] = empty ? -INFINITY : st.m + log_s;
-    if (p.entropies) p.entropies[slot] = empty ? 0.0f : log_s - st.u / st.s;
+    if (p.entropies) p.entropies[slot] = empty ? 0.0f : log_s - (st.u / st.s * TS_LN2 - r);
   }
-  ts_rank(lv, li, lists, k, tid - group * wpr * 32, wpr * 32, [&](int r, float v, uint32_t id) {
-    if (p.top_ids) p.top_ids[slot * k + r] = id;
-    if (p.top_log_probs) p.top_log_probs[slot * k + r] = empty ? -INFINITY : (v - st.m) - log_s;
-  });
+  if (k == 0) return;
+  const uint64_t key = lane < k ? sm.final[group][lane] : 0;
+  uint32_t id = ~(uint32_t)key;
+  const float v = key ? ts_value((uint32_t)(key >> 32)) : -INFINITY;
+  const int left = __popc(__ballot_sync(0xffffffffu, key != 0));
+  if (left < k) {
+    // Fewer unmasked columns than places: the lowest ids that are not among them.
+    uint64_t missing = columns >= 64 ? ~0ull : (1ull << columns) - 1;
+    for (int i = 0; i < left; ++i) {
+      const uint32_t taken = __shfl_sync(0xffffffffu, id, i);
+      if (taken < 64) missing &= ~(1ull << taken);
+    }
+    for (int i = left; i < lane; ++i) missing &= missing - 1;
+    if (lane >= left) id = (uint32_t)__ffsll((long long)missing) - 1;
+  }
+  if (lane < k) {
+    if (p.top_ids) p.top_ids[slot * k + lane] = id;
+    if (p.top_log_probs) p.top_log_probs[slot * k + lane] = empty ? -INFINITY : (v - st.m) - log_s;
+  }
 }
 
-template <typename T>
-int launch_typed(const DeviceCtx& dev, const TsParams& p, cudaStream_t stream) {
-  // Tiles of the longest row.
-  const int64_t vec = 16 / sizeof(T);
-  const int64_t tiles = (p.columns + 2 * vec - 2) / vec / (32 * TS_UNR) + 1;
-  int wpr = 1;
-  while (wpr < TS_WARPS && wpr < tiles) wpr *= 2;
-  int cluster = 1;
-  if (wpr == TS_WARPS)
-    while (cluster < TS_CLUSTER && p.rows * cluster * 2 <= dev.sm_count && tiles >= (int64_t)cluster * 2 * TS_WARPS)
-      cluster *= 2;
+template <typename T, int NV>
+int launch_route(const TsParams& p, int wpr, int cluster, cudaStream_t stream) {
   if (cluster > 1) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
@@ -430,12 +595,38 @@ int launch_typed(const DeviceCtx& dev, const TsParams& p, cudaStream_t stream) {
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cuda_error(cudaLaunchKernelEx(&cfg, token_scores_kernel<T, true>, p, (int)TS_WARPS), "token_scores launch");
+    return cuda_error(cudaLaunchKernelEx(&cfg, token_scores_kernel<T, NV, true>, p, (int)TS_WARPS), "token_scores launch");
   }
   const int64_t per = TS_WARPS / wpr;
-  return cuda_error(launch_kernel(token_scores_kernel<T, false>, dim3((unsigned)((p.rows + per - 1) / per)),
+  return cuda_error(launch_kernel(token_scores_kernel<T, NV, false>, dim3((unsigned)((p.rows + per - 1) / per)),
                                   dim3(TS_THREADS), 0, stream, p, wpr),
                     "token_scores launch");
+}
+
+template <typename T>
+int launch_typed(const DeviceCtx& dev, const TsParams& p, cudaStream_t stream) {
+  constexpr int64_t vec = 16 / sizeof(T);
+  const int64_t vectors = (p.columns + 2 * vec - 2) / vec;  // of the row with the worst start
+  auto warps_for = [&](int nv) {
+    int64_t w = 1;
+    while (w * 32 * nv < vectors) w *= 2;
+    return w;
+  };
+  // Few rows: every warp holds little, over as many SMs as there are.
+  int64_t few = warps_for(TS_HELD_FEW);
+  if (p.k > 16) few = std::max<int64_t>(few, 2);
+  if (few <= TS_WARPS * TS_CLUSTER && p.rows * few <= (int64_t)dev.sm_count * TS_WARPS)
+    return launch_route<T, TS_HELD_FEW>(p, (int)std::min<int64_t>(few, TS_WARPS), (int)std::max<int64_t>(1, few / TS_WARPS),
+                                        stream);
+  int64_t held = warps_for(TS_HELD);
+  // More alternatives than half a warp's lanes: 32 lane maxima would bound them too loosely.
+  if (p.k > 16) held = std::max<int64_t>(held, 2);
+  if (held <= TS_WARPS) return launch_route<T, TS_HELD>(p, (int)held, 1, stream);
+  if (held <= TS_WARPS * TS_CLUSTER && p.rows * held <= (int64_t)dev.sm_count * TS_WARPS)
+    return launch_route<T, TS_HELD>(p, TS_WARPS, (int)(held / TS_WARPS), stream);
+  int cluster = 1;
+  while (cluster < TS_CLUSTER && p.rows * cluster * 2 <= dev.sm_count) cluster *= 2;
+  return launch_route<T, 0>(p, TS_WARPS, cluster, stream);
 }
 
 }  // namespace
