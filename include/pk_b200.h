@@ -288,18 +288,19 @@ typedef struct pk_residual_norm_desc {
 int pk_residual_norm(pk_device* device, const pk_residual_norm_desc* desc, pk_stream stream);
 
 /* A few rows times a matrix held in 4 bits, the decode form of the palette
- * GEMM: C = epilogue(A . W), W[k, n] = (code[k, n] - 8) * scales[k / group, n].
+ * GEMM: C = epilogue(A . W), W[k, n] = (code[k, n] - 8) * scale[k / group, n].
  * The scale multiplies the group's f32 sum.  Epilogue as in pk_gemm_desc; bias
  * and residual are exclusive.  Codes lie in tiles of 16 outputs x 128 inputs
  * ("n16-k128-lane-major-int4-u32"): u32 [ceil(N / 16)][ceil(K / 128)][2][32][4],
  * where word i of lane l in half h holds, lowest bits first, the codes of
  * inputs 128 kt + 32 i + 8 (l % 4) + 0..7 of output 16 nt + 8 h + l / 4; places
- * outside the matrix hold code 8. */
+ * outside the matrix hold code 8.  Scales lie as
+ * [ceil(N / 16)][K / group][16] ("n16-k-group-major-scale"), zero outside. */
 typedef struct pk_int4_gemv_desc {
   int precision;             /* PK_FP16: A/C/residual/scales f16; PK_FP32: all f32 */
   int64_t rows;              /* 1..64 */
-  int64_t inner;             /* K, a multiple of 32 */
-  int64_t columns;           /* N */
+  int64_t inner;             /* K, a multiple of 32, at most 2^18 */
+  int64_t columns;           /* N, at most 2^22 */
   int64_t group;             /* inputs per scale: 32, 64 or a multiple of 128; divides K */
   int activation;            /* PK_ACT_* */
   float residual_scale;
@@ -307,7 +308,7 @@ typedef struct pk_int4_gemv_desc {
   const void* residual;      /* device [rows, N] or NULL: C = residual + residual_scale * value; may be C */
   const void* a;             /* device [rows, K], 16-byte aligned */
   const uint32_t* codes;     /* device, 16-byte aligned */
-  const void* scales;        /* device [K / group, N] */
+  const void* scales;        /* device [ceil(N / 16), K / group, 16] */
   void* c;                   /* device [rows, N] */
 } pk_int4_gemv_desc;
 int pk_int4_gemv(pk_device* device, const pk_int4_gemv_desc* desc, pk_stream stream);

@@ -432,7 +432,7 @@ int pk_int4_gemv(pk_device* device, const pk_int4_gemv_desc* d, pk_stream stream
   if (!device || !d || !d->a || !d->codes || !d->scales || !d->c) return set_error(PK_E_INVALID, "null argument");
   if (d->precision != PK_FP16 && d->precision != PK_FP32) return set_error(PK_E_INVALID, "unknown precision");
   if (d->rows < 1 || d->rows > 64) return set_error(PK_E_SHAPE, "int4 products take 1..64 rows, got %lld", (long long)d->rows);
-  if (d->inner <= 0 || d->inner % 32 != 0 || d->inner > (1 << 20) || d->columns <= 0 || d->columns > (1 << 22))
+  if (d->inner <= 0 || d->inner % 32 != 0 || d->inner > (1 << 18) || d->columns <= 0 || d->columns > (1 << 22))
     return set_error(PK_E_SHAPE, "Unsupported int4 shape: K=%lld N=%lld (needs K%%32==0)", (long long)d->inner,
                      (long long)d->columns);
   if (d->group <= 0 || d->inner % d->group != 0 || (d->group != 32 && d->group != 64 && d->group % 128 != 0))

@@ -14,17 +14,28 @@
 // warp's lanes hold the matrix operand, so a lane reads two 16-byte words per
 // tile and a warp 512 contiguous bytes at a time, four tiles ahead.  Word i of
 // a lane holds inputs 32 i + 8 t .. + 7 (t = lane % 4) of outputs lane / 4 (+ 8
-// in the second 16 bytes).  A code becomes f16 by placing its 4 bits in the
-// mantissa of 1024 (or, 4 bits further up, as 16 times the code) and
-// subtracting: 9 instructions for 8 weights, exact.  That makes pairs of inputs
-// (0,4) (1,5) (2,6) (3,7); A's rows lie in shared memory in that order.
+// in the second 16 bytes).  A code becomes f16 by placing its 4 bits in a
+// mantissa: 1024 + code where they are the lowest, less 1032 in one more
+// instruction; 64 + code where they are the next four, which stays as it is --
+// the sums of a group begin at -72 times the sum of those inputs instead (the
+// first product's addend).  7 instructions for 8 weights; the second form adds
+// values 16 times the weights' size to the f32 sums, 2^-20 of a product's size.
+// That makes pairs of inputs (0,4) (1,5) (2,6) (3,7); A's rows lie in shared
+// memory in that order.
 //
 // The scale multiplies a group's f32 sum, not the weight: no weight is
 // rounded.  FP32 rows are two f16 columns each, the leading 11 bits and the
 // next 11, after a power-of-two scale per row and 128 inputs that brings the
 // largest to [2^14, 2^15): 22 bits of every input, where the sum's own rounding
-// is 24.  The warps of a CTA split outputs and inputs; the inputs' parts join
-// in shared memory in a fixed order (no atomics).
+// is 24.
+//
+// One CTA per SM walks the output tiles; A's rows are laid out in its shared
+// memory once.  Its warps split outputs (wm) and inputs (wk), so that the
+// outputs of an SM come out even: 1024 tiles on 148 SMs are 7 a SM, at once.
+// Where the rows are more than shared memory holds, or the outputs are fewer
+// than the SMs, a cluster of CTAs splits the inputs and joins through
+// distributed shared memory.  Parts join in a fixed order: no workspace, no
+// atomics.
 #include <algorithm>
 
 #include "pk_common.cuh"
@@ -33,11 +44,14 @@
 namespace pk {
 namespace {
 
-constexpr int I4_WARPS = 8;       // warps per CTA, at most
 constexpr int I4_KT = 128;        // inputs per tile
-constexpr int I4_DEPTH = 4;       // tiles in flight per warp
-constexpr int I4_COLS = 64;       // columns of one pass, at most
-constexpr int I4_STAGE_BYTES = 72 * 1024;  // shared memory for A's rows, about
+constexpr int I4_COLS = 32;       // columns of one pass, at most (more rows: the codes again, from L2)
+constexpr int I4_CLUSTER = 8;     // CTAs that share the inputs, at most
+constexpr int I4_SMEM = 220 * 1024;
+
+// Warps per CTA (registers: 72, 96, 128 a thread) and tiles in flight per warp.
+__host__ __device__ constexpr int i4_warps(int nt) { return nt == 1 ? 28 : nt == 2 ? 20 : 16; }
+__host__ __device__ constexpr int i4_depth(int gb) { return gb < 4 ? 2 : 3; }
 
 struct I4Params {
   const void* a;
@@ -46,10 +60,14 @@ struct I4Params {
   const float* bias;
   const void* residual;
   void* c;
-  int rows, inner, columns, ktiles, group, groups;
-  int wm, wk;        // warps over outputs, over inputs
-  int chunk;         // tiles of A staged at a time (a multiple of wk * I4_DEPTH, or all)
+  int rows, inner, columns, ktiles;
+  int groups;           // scales per output
+  uint32_t group_inv;   // 2^32 / (tiles per group), rounded up (groups of whole tiles)
+  int wm, wk;           // warps over outputs, over inputs
+  int ktiles_cta;       // tiles of inputs per CTA of a cluster
+  int cluster;
   int rows_per_pass;
+  int part_offset;      // bytes of shared memory before the parts
   int act;
   float residual_scale;
 };
@@ -62,14 +80,14 @@ __device__ __forceinline__ uint32_t i4_lop(uint32_t a, uint32_t b, uint32_t c) {
 __device__ __forceinline__ uint32_t i4_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 i4_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
-// Eight codes -> four pairs (0,4) (1,5) (2,6) (3,7) of code - 8.
+// Eight codes -> the pairs (0,4) (2,6) of code - 8 and (1,5) (3,7) of code + 64.
 __device__ __forceinline__ void i4_expand(uint32_t w, uint32_t (&p)[4]) {
-  const __half2 one = __float2half2_rn(1032.0f), sixteenth = __float2half2_rn(0.0625f), off = __float2half2_rn(-72.0f);
+  const __half2 off = __float2half2_rn(1032.0f);
   const uint32_t w8 = w >> 8;
-  p[0] = i4_bits(__hsub2(i4_h2(i4_lop(w, 0x000f000fu, 0x64006400u)), one));
-  p[1] = i4_bits(__hfma2(i4_h2(i4_lop(w, 0x00f000f0u, 0x64006400u)), sixteenth, off));
-  p[2] = i4_bits(__hsub2(i4_h2(i4_lop(w8, 0x000f000fu, 0x64006400u)), one));
-  p[3] = i4_bits(__hfma2(i4_h2(i4_lop(w8, 0x00f000f0u, 0x64006400u)), sixteenth, off));
+  p[0] = i4_bits(__hsub2(i4_h2(i4_lop(w, 0x000f000fu, 0x64006400u)), off));
+  p[1] = i4_lop(w, 0x00f000f0u, 0x54005400u);
+  p[2] = i4_bits(__hsub2(i4_h2(i4_lop(w8, 0x000f000fu, 0x64006400u)), off));
+  p[3] = i4_lop(w8, 0x00f000f0u, 0x54005400u);
 }
 
 __device__ __forceinline__ void i4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -77,6 +95,14 @@ __device__ __forceinline__ void i4_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// D = A B + C: the first product of a group's sum.
+__device__ __forceinline__ void i4_mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1, float4 c) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
 }
 
 __device__ __forceinline__ uint4 i4_load(const uint4* p) {
@@ -89,28 +115,40 @@ __device__ __forceinline__ uint4 i4_load(const uint4* p) {
 
 // Bytes of one column of staged inputs: the columns of a quarter warp's loads
 // fall on different banks.
-__host__ __device__ inline int i4_col_bytes(int chunk) { return chunk * I4_KT * 2 + 64; }
+__host__ __device__ inline int i4_col_bytes(int ktiles) { return ktiles * I4_KT * 2 + 64; }
 
-// Stages tiles [kt0, kt0 + tiles) of `rows` rows of A: 16 lanes per row and
+// The addend of a group's first product, as a lane holds it: -72 times the
+// sums of the inputs that meet code + 64, columns 2 t and 2 t + 1 twice.
+// [tile of inputs][scale of the tile][column / 2] float4.
+template <int NT>
+__device__ __forceinline__ float* i4_addend(float* base, int block, int col) {
+  return base + (size_t)(block * NT * 4 + (col >> 1)) * 4 + (col & 1);
+}
+
+// Lays out tiles [kt0, kt0 + tiles) of `rows` rows of A: 16 lanes per row and
 // tile, eight inputs each, in the order 0 4 1 5 2 6 3 7.
-template <typename T>
-__device__ __forceinline__ void i4_stage(const I4Params& p, unsigned char* xs, float* xscale, int row0, int rows, int kt0,
-                                         int tiles) {
+template <typename T, int NT, int GB>
+__device__ __forceinline__ void i4_stage(const I4Params& p, unsigned char* xs, float* xscale, float* addend, int row0,
+                                         int rows, int kt0, int tiles) {
+  constexpr int PARTS = sizeof(T) == 2 ? 1 : 2;
+  constexpr int SPT = 4 / GB;
   const int lane16 = threadIdx.x & 15;
   const int jobs = rows * tiles;
-  const int stride = i4_col_bytes(p.chunk);
-  for (int j0 = (threadIdx.x >> 5) * 2; j0 < jobs; j0 += (blockDim.x >> 5) * 2) {
-    const int j = j0 + ((threadIdx.x >> 4) & 1);  // the two halves of a warp
-    const int r = min(j, jobs - 1) / tiles, kt = min(j, jobs - 1) % tiles;
+  const int stride = i4_col_bytes(p.ktiles_cta);
+  const int halves = (blockDim.x >> 5) * 2;  // half warps of the CTA
+  for (int j0 = (threadIdx.x >> 5) * 2; j0 < jobs; j0 += halves) {
+    const int j = min(j0 + (int)((threadIdx.x >> 4) & 1), jobs - 1);
+    const bool mine = j0 + (int)((threadIdx.x >> 4) & 1) < jobs;
+    const int r = j / tiles, kt = j % tiles;
     const int k = (kt0 + kt) * I4_KT + 8 * lane16;
     const T* src = static_cast<const T*>(p.a) + (size_t)(row0 + r) * p.inner + k;
     const bool in = k < p.inner;  // inner is a multiple of 32: eight at once
-    if constexpr (sizeof(T) == 2) {
+    uint4 col[PARTS];
+    if constexpr (PARTS == 1) {
       uint4 v = make_uint4(0u, 0u, 0u, 0u);
       if (in) v = *reinterpret_cast<const uint4*>(src);
-      const uint4 o = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
-                                 __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-      if (j < jobs) *reinterpret_cast<uint4*>(xs + (size_t)r * stride + kt * (I4_KT * 2) + lane16 * 16) = o;
+      col[0] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                          __byte_perm(v.y, v.w, 0x7632));
     } else {
       float v[8] = {};
       if (in) {
@@ -134,214 +172,283 @@ __device__ __forceinline__ void i4_stage(const I4Params& p, unsigned char* xs, f
         // An infinite or NaN input stands in the first column alone.
         lo[i] = __float2half_rn(fabsf(h) <= 65504.0f ? y - h : 0.0f);
       }
-      if (j < jobs) {
-        const int at[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-        uint4 a, b;
-        __half* ha = reinterpret_cast<__half*>(&a);
-        __half* hb = reinterpret_cast<__half*>(&b);
+      const int at[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+      __half* ha = reinterpret_cast<__half*>(&col[0]);
+      __half* hb = reinterpret_cast<__half*>(&col[PARTS - 1]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          ha[i] = hi[at[i]];
-          hb[i] = lo[at[i]];
-        }
-        unsigned char* dst = xs + (size_t)(2 * r) * stride + kt * (I4_KT * 2) + lane16 * 16;
-        *reinterpret_cast<uint4*>(dst) = a;
-        *reinterpret_cast<uint4*>(dst + stride) = b;
-        if (lane16 == 0) xscale[r * p.chunk + kt] = down;
+      for (int i = 0; i < 8; ++i) {
+        ha[i] = hi[at[i]];
+        hb[i] = lo[at[i]];
+      }
+      if (mine && lane16 == 0) xscale[r * p.ktiles_cta + kt] = down;
+    }
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+      if (mine) *reinterpret_cast<uint4*>(xs + (size_t)(r * PARTS + q) * stride + kt * (I4_KT * 2) + lane16 * 16) = col[q];
+      // The second and fourth pairs of the eight; four lanes hold 32 inputs.
+      const float2 b = __half22float2(i4_h2(col[q].y)), d = __half22float2(i4_h2(col[q].w));
+      float sum = (b.x + b.y) + (d.x + d.y);
+#pragma unroll
+      for (int o = 1; o < 4 * GB; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (mine && lane16 % (4 * GB) == 0) {
+        float* dst = i4_addend<NT>(addend, kt * SPT + lane16 / (4 * GB), r * PARTS + q);
+        // An infinite sum would meet the products' infinities as a NaN; they need no addend.
+        const float v = fabsf(sum) <= 3.0e38f || sum != sum ? -72.0f * sum : 0.0f;
+        dst[0] = v;
+        dst[2] = v;
       }
     }
   }
 }
 
-// NT tiles of 8 columns, MT tiles of 16 outputs per warp, GB blocks of 32
-// inputs per scale within a tile (1, 2, or 4: groups of whole tiles).
-template <typename T, int NT, int MT, int GB>
-__global__ void __launch_bounds__(I4_WARPS * 32) int4_gemv_kernel(const I4Params p) {
+// NT tiles of 8 columns, GB blocks of 32 inputs per scale within a tile (1, 2,
+// or 4: groups of whole tiles).
+template <typename T, int NT, int GB>
+__global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I4Params p) {
   extern __shared__ __align__(128) unsigned char i4_smem[];
   constexpr int PARTS = sizeof(T) == 2 ? 1 : 2;  // columns per row
   constexpr int SPT = 4 / GB;                    // scales per tile and output
+  constexpr int DEPTH = i4_depth(GB);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int wm = warp % p.wm, wk = warp / p.wm;
+  const int wm = warp / p.wk, wk = warp % p.wk;
+  const int rank = p.cluster > 1 ? (int)cluster_ctarank() : 0;
   const int row0 = blockIdx.y * p.rows_per_pass;
   const int rows = min(p.rows - row0, p.rows_per_pass);
   const int cols = rows * PARTS;
-  const int mtile0 = (blockIdx.x * p.wm + wm) * MT;  // this warp's first tile of 16 outputs
   const int mtiles = (p.columns + 15) / 16;
+  const int walk = (int)gridDim.x / p.cluster * p.wm;  // tiles of outputs between a warp's
+  const int k0 = rank * p.ktiles_cta;                  // this CTA's tiles of inputs
+  const int ktiles = max(0, min(p.ktiles_cta, p.ktiles - k0));
   unsigned char* xs = i4_smem;
-  const int stride = i4_col_bytes(p.chunk);
-  float* xscale = reinterpret_cast<float*>(i4_smem + (size_t)cols * stride);
+  const int stride = i4_col_bytes(p.ktiles_cta);
+  float* addend = reinterpret_cast<float*>(i4_smem + (size_t)cols * stride);
+  float* xscale = addend + (size_t)p.ktiles_cta * SPT * NT * 16;
 
   struct Slot {
-    uint4 code[MT][2];
-    T scale[MT][2][SPT];
+    uint4 code[2];
+    T scale[2][SPT];
   };
-  Slot ring[I4_DEPTH];
-  auto load = [&](Slot& s, int kt) {
-    if (kt >= p.ktiles) return;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int mt = min(mtile0 + m, mtiles - 1);
-      const uint4* src = p.codes + ((size_t)mt * p.ktiles + kt) * 64 + lane;
-      s.code[m][0] = i4_load(src);
-      s.code[m][1] = i4_load(src + 32);
+  Slot ring[DEPTH];
+  // What is loaded next: this warp's tile `lk` of inputs (of the CTA's) for
+  // output tile `lm`.  A warp's tiles come in rounds of DEPTH, the last of them
+  // perhaps empty.
+  const int rounds = (p.ktiles_cta + p.wk * DEPTH - 1) / (p.wk * DEPTH);
+  const int round_end = wk + rounds * DEPTH * p.wk;
+  const int first = (int)blockIdx.x / p.cluster * p.wm + wm;
+  int lm = first, lk = wk, lend = first < mtiles ? ktiles : 0;
+  const uint4* lcode;
+  const T* lscale;
+  auto aim = [&]() {
+    lcode = p.codes + ((size_t)lm * p.ktiles + k0 + lk) * 64 + lane;
+    lscale = static_cast<const T*>(p.scales) + (size_t)lm * p.groups * 16 + g;
+  };
+  aim();
+  auto load = [&](Slot& s) {
+    if (lk < lend) {
+      s.code[0] = i4_load(lcode);
+      s.code[1] = i4_load(lcode + 32);
+      const int kt = k0 + lk;
 #pragma unroll
       for (int b = 0; b < SPT; ++b) {
-        const int gi = min((kt * I4_KT + b * GB * 32) / p.group, p.groups - 1);
-        const T* sc = static_cast<const T*>(p.scales) + (size_t)gi * p.columns;
-        s.scale[m][0][b] = __ldg(sc + min(mt * 16 + g, p.columns - 1));
-        s.scale[m][1][b] = __ldg(sc + min(mt * 16 + g + 8, p.columns - 1));
+        const int gi = GB == 4 ? (p.group_inv ? (int)__umulhi((uint32_t)kt, p.group_inv) : kt) : min(kt * SPT + b, p.groups - 1);
+        s.scale[0][b] = __ldg(lscale + gi * 16);
+        s.scale[1][b] = __ldg(lscale + gi * 16 + 8);
       }
+    }
+    lk += p.wk;
+    lcode += p.wk * 64;
+    if (lk == round_end) {
+      lk = wk;
+      lm += walk;
+      if (lm >= mtiles) lend = 0;
+      aim();
     }
   };
   // The weights too may be the previous kernel's work (a pack, a load): nothing
   // is read before it is done.
   pdl_entry();
 #pragma unroll
-  for (int d = 0; d < I4_DEPTH; ++d) load(ring[d], wk + d * p.wk);
+  for (int d = 0; d < DEPTH; ++d) load(ring[d]);
+  i4_stage<T, NT, GB>(p, xs, xscale, addend, row0, rows, k0, ktiles);
+  __syncthreads();
 
-  float total[MT][NT][4] = {};
   const unsigned char* xcol[NT];
-  int xrow[NT][2];
+  const float* xsc[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     xcol[n] = xs + (size_t)min(n * 8 + g, cols - 1) * stride + t * 16;
-    xrow[n][0] = min((n * 8 + 2 * t) / PARTS, rows - 1) * p.chunk;
-    xrow[n][1] = min((n * 8 + 2 * t + 1) / PARTS, rows - 1) * p.chunk;
+    xsc[n] = xscale + min(n * 4 + t, rows - 1) * p.ktiles_cta;  // FP32: columns 2 t and 2 t + 1 are one row
   }
-  for (int kt0 = 0; kt0 < p.ktiles; kt0 += p.chunk) {
-    const int tiles = min(p.chunk, p.ktiles - kt0);
-    if (kt0) __syncthreads();
-    i4_stage<T>(p, xs, xscale, row0, rows, kt0, tiles);
-    __syncthreads();
-    for (int k1 = wk; k1 < tiles; k1 += I4_DEPTH * p.wk) {
+  const int M = p.wm * 16;
+  constexpr int PC = NT * 8;
+  float* part = reinterpret_cast<float*>(i4_smem + p.part_offset);  // [wk][column][output]
+  float* sums = part + (size_t)p.wk * PC * (M + 4);                 // cluster: [parity][row][output]
+  const int pm = tid % M, pr = tid / M;  // the output and first row that this thread joins (2 wk threads per output)
+  int parity = 0;
+  for (int m0 = (int)blockIdx.x / p.cluster * p.wm; m0 < mtiles; m0 += walk, parity ^= 1) {
+    float total[NT][4] = {};
+    for (int r = 0; r < rounds; ++r) {
 #pragma unroll
-      for (int d = 0; d < I4_DEPTH; ++d) {
-        const int kl = k1 + d * p.wk;  // tile of the chunk
-        if (kl < tiles) {
-          Slot& s = ring[d];
+      for (int d = 0; d < DEPTH; ++d) {
+        const int kl = wk + (r * DEPTH + d) * p.wk;
+        Slot& s = ring[d];
+        if (kl < ktiles && m0 + wm < mtiles) {
 #pragma unroll
           for (int b = 0; b < SPT; ++b) {
-            float acc[MT][NT][4] = {};
+            float acc[NT][4];
 #pragma unroll
             for (int i = b * GB; i < (b + 1) * GB; ++i) {
               uint4 x[NT];
 #pragma unroll
               for (int n = 0; n < NT; ++n)
                 x[n] = *reinterpret_cast<const uint4*>(xcol[n] + kl * (I4_KT * 2) + i * 64);
+              uint32_t w0[4], w1[4];
+              i4_expand((&s.code[0].x)[i], w0);
+              i4_expand((&s.code[1].x)[i], w1);
 #pragma unroll
-              for (int m = 0; m < MT; ++m) {
-                uint32_t w0[4], w1[4];
-                i4_expand((&s.code[m][0].x)[i], w0);
-                i4_expand((&s.code[m][1].x)[i], w1);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                  i4_mma(acc[m][n], w0[0], w1[0], w0[1], w1[1], x[n].x, x[n].y);
-                  i4_mma(acc[m][n], w0[2], w1[2], w0[3], w1[3], x[n].z, x[n].w);
-                }
+              for (int n = 0; n < NT; ++n) {
+                if (i == b * GB)
+                  i4_mma_first(acc[n], w0[0], w1[0], w0[1], w1[1], x[n].x, x[n].y,
+                               *reinterpret_cast<const float4*>(addend + (size_t)((kl * SPT + b) * NT * 4 + n * 4 + t) * 4));
+                else
+                  i4_mma(acc[n], w0[0], w1[0], w0[1], w1[1], x[n].x, x[n].y);
+                i4_mma(acc[n], w0[2], w1[2], w0[3], w1[3], x[n].z, x[n].w);
               }
             }
+            const float s0 = (float)s.scale[0][b], s1 = (float)s.scale[1][b];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              float x0 = 1.0f, x1 = 1.0f;
+              float f0 = s0, f1 = s1;
               if constexpr (PARTS == 2) {
-                x0 = xscale[xrow[n][0] + kl];
-                x1 = xscale[xrow[n][1] + kl];
+                const float f = xsc[n][kl];
+                f0 *= f;
+                f1 *= f;
               }
-#pragma unroll
-              for (int m = 0; m < MT; ++m) {
-                const float s0 = (float)s.scale[m][0][b], s1 = (float)s.scale[m][1][b];
-                total[m][n][0] = fmaf(s0 * x0, acc[m][n][0], total[m][n][0]);
-                total[m][n][1] = fmaf(s0 * x1, acc[m][n][1], total[m][n][1]);
-                total[m][n][2] = fmaf(s1 * x0, acc[m][n][2], total[m][n][2]);
-                total[m][n][3] = fmaf(s1 * x1, acc[m][n][3], total[m][n][3]);
-              }
+              total[n][0] = fmaf(f0, acc[n][0], total[n][0]);
+              total[n][1] = fmaf(f0, acc[n][1], total[n][1]);
+              total[n][2] = fmaf(f1, acc[n][2], total[n][2]);
+              total[n][3] = fmaf(f1, acc[n][3], total[n][3]);
             }
           }
-          load(s, kt0 + kl + I4_DEPTH * p.wk);
         }
+        load(s);
       }
     }
-  }
-  // Parts of the inputs' split, [wk][column][output]: the staged rows are done with.
-  __syncthreads();
-  const int M = p.wm * MT * 16;
-  constexpr int PC = NT * 8;
-  float* part = reinterpret_cast<float*>(i4_smem);
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        part[((size_t)wk * PC + n * 8 + 2 * t + (e & 1)) * (M + 4) + (wm * MT + m) * 16 + g + 8 * (e >> 1)] =
-            total[m][n][e];
-  __syncthreads();
-  for (int i = tid; i < rows * M; i += blockDim.x) {
-    const int r = i / M, m = i % M;
-    const int n = blockIdx.x * M + m;
-    if (n >= p.columns) continue;
-    float v = 0.0f;
-    for (int w = 0; w < p.wk; ++w)
+        part[((size_t)wk * PC + n * 8 + 2 * t + (e & 1)) * (M + 4) + wm * 16 + g + 8 * (e >> 1)] = total[n][e];
+    __syncthreads();
+    auto finish = [&](int r, int n, float v) {
+      if (n >= p.columns) return;
+      if (p.bias) v += __ldg(p.bias + n);
+      if (p.act == PK_ACT_SILU) v = v / (1.0f + expf(-v));
+      else if (p.act == PK_ACT_RELU) v = v < 0.0f ? 0.0f : v;
+      const size_t at = (size_t)(row0 + r) * p.columns + n;
+      if (p.residual) v = fmaf(p.residual_scale, v, (float)static_cast<const T*>(p.residual)[at]);
+      static_cast<T*>(p.c)[at] = (T)v;
+    };
+    for (int r = pr; r < rows; r += 2 * p.wk) {
+      float v = 0.0f;
+      const float* src = part + (size_t)r * PARTS * (M + 4) + pm;
+      for (int w = 0; w < p.wk; ++w, src += PC * (M + 4)) {
+        v += src[0];
+        if constexpr (PARTS == 2) v += src[M + 4];
+      }
+      if (p.cluster == 1) finish(r, m0 * 16 + pm, v);
+      else sums[(size_t)(parity * rows + r) * M + pm] = v;
+    }
+    __syncthreads();  // the parts are read (and the sums written)
+    if (p.cluster > 1) {
+      // Each CTA finishes its share of the rows.  The sums of this parity are
+      // written again two tiles on, behind the next tile's barrier.
+      cluster_sync();
+      for (int r = pr * p.cluster + rank; r < rows; r += 2 * p.wk * p.cluster) {
+        const uint32_t at = smem_addr(sums + (size_t)(parity * rows + r) * M + pm);
+        float u[I4_CLUSTER];
 #pragma unroll
-      for (int q = 0; q < PARTS; ++q) v += part[((size_t)w * PC + r * PARTS + q) * (M + 4) + m];
-    if (p.bias) v += __ldg(p.bias + n);
-    if (p.act == PK_ACT_SILU) v = v / (1.0f + expf(-v));
-    else if (p.act == PK_ACT_RELU) v = v < 0.0f ? 0.0f : v;
-    const size_t at = (size_t)(row0 + r) * p.columns + n;
-    if (p.residual) v = fmaf(p.residual_scale, v, (float)static_cast<const T*>(p.residual)[at]);
-    static_cast<T*>(p.c)[at] = (T)v;
+        for (int c = 0; c < I4_CLUSTER; ++c)
+          if (c < p.cluster) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(u[c]) : "r"(mapa_shared(at, (uint32_t)c)));
+        float v = 0.0f;
+#pragma unroll
+        for (int c = 0; c < I4_CLUSTER; ++c)
+          if (c < p.cluster) v += u[c];
+        finish(r, m0 * 16 + pm, v);
+      }
+    }
+  }
+  if (p.cluster > 1) {
+    __syncwarp();
+    cluster_sync();  // no CTA leaves while another reads its sums
   }
 }
 
-template <typename T, int NT, int MT, int GB>
+template <typename T, int NT, int GB>
 int launch_one(const I4Params& p, dim3 grid, int smem, cudaStream_t stream) {
-  if (smem > 48 * 1024) {
-    const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(int4_gemv_kernel<T, NT, MT, GB>), 200 * 1024);
-    if (st != PK_OK) return st;
-  }
-  return cuda_error(launch_kernel(int4_gemv_kernel<T, NT, MT, GB>, grid, dim3((unsigned)(p.wm * p.wk * 32)),
-                                  (size_t)smem, stream, p),
-                    "int4_gemv launch");
+  const void* kernel = reinterpret_cast<const void*>(int4_gemv_kernel<T, NT, GB>);
+  const int st = set_max_dynamic_smem(kernel, I4_SMEM);
+  if (st != PK_OK) return st;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)(p.wm * p.wk * 32));
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.cluster > 1 ? 2 : 1;
+  return cuda_error(cudaLaunchKernelEx(&cfg, int4_gemv_kernel<T, NT, GB>, p), "int4_gemv launch");
 }
 
-template <typename T, int NT, int MT>
-int launch_group(const I4Params& p, dim3 grid, int smem, cudaStream_t stream) {
-  if (p.group == 32) return launch_one<T, NT, MT, 1>(p, grid, smem, stream);
-  if (p.group == 64) return launch_one<T, NT, MT, 2>(p, grid, smem, stream);
-  return launch_one<T, NT, MT, 4>(p, grid, smem, stream);
+template <typename T, int NT>
+int launch_group(const I4Params& p, int group, dim3 grid, int smem, cudaStream_t stream) {
+  if (group == 32) return launch_one<T, NT, 1>(p, grid, smem, stream);
+  if (group == 64) return launch_one<T, NT, 2>(p, grid, smem, stream);
+  return launch_one<T, NT, 4>(p, grid, smem, stream);
 }
 
 template <typename T>
-int launch_typed(const DeviceCtx& dev, I4Params p, cudaStream_t stream) {
+int launch_typed(const DeviceCtx& dev, I4Params p, int group, cudaStream_t stream) {
   constexpr int PARTS = sizeof(T) == 2 ? 1 : 2;
-  p.rows_per_pass = std::min(p.rows, I4_COLS / PARTS);
-  const int passes = (p.rows + p.rows_per_pass - 1) / p.rows_per_pass;
-  const int cols = p.rows_per_pass * PARTS;
-  const int nt = cols <= 8 ? 1 : cols <= 16 ? 2 : cols <= 32 ? 4 : 8;
-  const int mt = nt == 4 ? 2 : 1;
   const int mtiles = (p.columns + 15) / 16;
-  // Warps over the inputs: as many as there are tiles for, and as the staged
-  // rows leave room for with I4_DEPTH tiles each.
-  int wk = 1;
-  while (wk < I4_WARPS && 2 * wk <= p.ktiles && 2 * wk * I4_DEPTH * I4_KT * 2 * cols <= I4_STAGE_BYTES) wk *= 2;
-  int wm = I4_WARPS / wk;
-  // Outputs rather than inputs where there are enough of them for every SM.
-  while (wk > 1 && (mtiles + 2 * wm * mt - 1) / (2 * wm * mt) >= 2 * dev.sm_count) wk /= 2, wm *= 2;
-  while (wm > 1 && (mtiles + wm * mt - 1) / (wm * mt) < dev.sm_count) wm /= 2;
-  p.wm = wm;
-  p.wk = wk;
-  const int step = wk * I4_DEPTH;
-  p.chunk = std::max(step, I4_STAGE_BYTES / (cols * I4_KT * 2) / step * step);
-  if (p.chunk >= p.ktiles) p.chunk = p.ktiles;
-  const int stage = cols * i4_col_bytes(p.chunk) + (PARTS == 2 ? p.rows_per_pass * p.chunk * 4 : 0);
-  const int parts = wk * nt * 8 * (wm * mt * 16 + 4) * 4;
-  const int smem = std::max(stage, parts);
-  const dim3 grid((unsigned)((mtiles + wm * mt - 1) / (wm * mt)), (unsigned)passes);
-  if (nt == 1) return launch_group<T, 1, 1>(p, grid, smem, stream);
-  if (nt == 2) return launch_group<T, 2, 1>(p, grid, smem, stream);
-  if (nt == 4) return launch_group<T, 4, 2>(p, grid, smem, stream);
-  return launch_group<T, 8, 1>(p, grid, smem, stream);
+  int cols = std::min(p.rows * PARTS, I4_COLS);
+  int nt = 0, smem = 0;
+  // Columns per pass, then CTAs per cluster: the least that fit.
+  for (;; cols = std::max(PARTS, cols / 2 / PARTS * PARTS)) {
+    p.rows_per_pass = cols / PARTS;
+    nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
+    const int warps = i4_warps(nt);
+    for (p.cluster = 1; p.cluster <= I4_CLUSTER; p.cluster *= 2) {
+      // Few outputs: the inputs over more SMs, while each has a tile for every warp of 4.
+      if (mtiles * p.cluster * 2 <= dev.sm_count && p.cluster < I4_CLUSTER && p.ktiles >= p.cluster * 2 * 4) continue;
+      p.ktiles_cta = (p.ktiles + p.cluster - 1) / p.cluster;
+      const int clusters = dev.sm_count / p.cluster;
+      const int q = (mtiles + clusters - 1) / clusters;  // output tiles of a cluster
+      const int turns = (q + warps - 1) / warps;
+      p.wm = (q + turns - 1) / turns;
+      p.wk = std::max(1, std::min(p.ktiles_cta, warps / p.wm));
+      const int spt = group == 32 ? 4 : group == 64 ? 2 : 1;
+      p.part_offset = cols * i4_col_bytes(p.ktiles_cta) + p.ktiles_cta * spt * nt * 64;
+      p.part_offset = (p.part_offset + (PARTS == 2 ? p.rows_per_pass * p.ktiles_cta * 4 : 0) + 127) / 128 * 128;
+      smem = p.part_offset + p.wk * nt * 8 * (p.wm * 16 + 4) * 4 + (p.cluster > 1 ? 2 * p.rows_per_pass * p.wm * 16 * 4 : 0);
+      if (smem <= I4_SMEM) break;
+    }
+    if (p.cluster <= I4_CLUSTER || cols == PARTS) break;
+  }
+  if (smem > I4_SMEM) return set_error(PK_E_SHAPE, "int4 products of K=%d do not fit shared memory", p.inner);
+  const int passes = (p.rows + p.rows_per_pass - 1) / p.rows_per_pass;
+  const int clusters = std::min(dev.sm_count / p.cluster, (mtiles + p.wm - 1) / p.wm);
+  const dim3 grid((unsigned)(clusters * p.cluster), (unsigned)passes);
+  if (nt == 1) return launch_group<T, 1>(p, group, grid, smem, stream);
+  if (nt == 2) return launch_group<T, 2>(p, group, grid, smem, stream);
+  return launch_group<T, 4>(p, group, grid, smem, stream);
 }
 
 }  // namespace
@@ -358,11 +465,14 @@ int launch_int4_gemv(const DeviceCtx& dev, const pk_int4_gemv_desc& d, cudaStrea
   p.inner = (int)d.inner;
   p.columns = (int)d.columns;
   p.ktiles = (int)((d.inner + I4_KT - 1) / I4_KT);
-  p.group = (int)d.group;
   p.groups = (int)(d.inner / d.group);
+  // Exact for fewer than 2^13 tiles; 0: one tile per group.
+  const int per = (int)(d.group / I4_KT);
+  p.group_inv = per > 1 ? (uint32_t)((((uint64_t)1 << 32) + per - 1) / per) : 0u;
   p.act = d.activation;
   p.residual_scale = d.residual_scale;
-  return d.precision == PK_FP16 ? launch_typed<__half>(dev, p, stream) : launch_typed<float>(dev, p, stream);
+  return d.precision == PK_FP16 ? launch_typed<__half>(dev, p, (int)d.group, stream)
+                                : launch_typed<float>(dev, p, (int)d.group, stream);
 }
 
 }  // namespace pk

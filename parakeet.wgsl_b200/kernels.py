@@ -838,7 +838,7 @@ class Int4Weight:
     @staticmethod
     def from_words(words, scales, inner: int, group: int, name: str = "int4") -> "Int4Weight":
         """words: CUDA int32 / uint32 [N, K / 8] (rp.INT4_LAYOUT), scales: CUDA f16 or f32
-        [K / group, N].  The re-laid codes are a copy; the scales are used as they are."""
+        [K / group, N].  Both are re-laid copies."""
         columns = int(words.shape[0])
         try:
             rp.check_int4_geometry(inner, columns, group)
@@ -858,10 +858,14 @@ class Int4Weight:
             w = full
         # [tile row, half, lane / 4, tile column, block of 32 inputs, lane % 4]
         tiles = w.reshape(nt, 2, 8, kt, 4, 4).permute(0, 3, 1, 2, 5, 4).contiguous().reshape(-1)
+        padded = torch.zeros((inner // group, nt * 16), dtype=scales.dtype, device=w.device) if columns % 16 else scales
+        if columns % 16:
+            padded[:, :columns] = scales
+        laid = padded.reshape(inner // group, nt, 16).permute(1, 0, 2).contiguous().reshape(-1)
         scalar = "float16" if scales.dtype == torch.float16 else "float32"
         return Int4Weight(inner, columns, group,
                           GpuTensor(f"{name}.codes", "uint32", (inner, columns), rp.INT4_TILE_LAYOUT, tiles),
-                          GpuTensor(f"{name}.scales", scalar, (inner // group, columns), rp.INT4_SCALE_LAYOUT, scales))
+                          GpuTensor(f"{name}.scales", scalar, (inner // group, columns), rp.INT4_TILE_SCALE_LAYOUT, laid))
 
     @staticmethod
     def quantize(weight: np.ndarray, group: int, profile: str = "fp16", device: str = "cuda",
@@ -894,7 +898,8 @@ class Int4GemvKernel:
         if rows > self.MAX_ROWS:
             raise RangeError(f"{label} rows must be in [1, {self.MAX_ROWS}]")
         scalar = _scalar_dtype(self.profile)
-        if not isinstance(w, Int4Weight) or w.codes.layout != rp.INT4_TILE_LAYOUT:
+        if (not isinstance(w, Int4Weight) or w.codes.layout != rp.INT4_TILE_LAYOUT
+                or w.scales.layout != rp.INT4_TILE_SCALE_LAYOUT):
             raise ParakeetError(f"{label} has an unsupported weight format")
         if w.scales.tensor.dtype != scalar:
             raise ParakeetError(f"{label} scales must be {scalar}, got {w.scales.tensor.dtype}")
@@ -910,7 +915,7 @@ class Int4GemvKernel:
         residual = _operand(d, "residual", scalar, rows * w.columns, dev, optional=True)
         own = {"codes": w.codes, "scales": w.scales, "label": label}
         codes = _operand(own, "codes", _ids(), -(-w.columns // 16) * -(-w.inner // 128) * 256, dev)
-        scales = _operand(own, "scales", scalar, w.inner // w.group * w.columns, dev)
+        scales = _operand(own, "scales", scalar, -(-w.columns // 16) * (w.inner // w.group) * 16, dev)
         scale = d.get("residual_scale")
         desc = _lib.Int4GemvDesc(_precision(self.profile), rows, w.inner, w.columns, w.group,
                                  _lib.ACT[d.get("activation", "none")], 1.0 if scale is None else float(scale),

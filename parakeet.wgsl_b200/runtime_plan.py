@@ -30,7 +30,7 @@ PALETTE6_LAYOUT = "k-by-output-row-major-palette6-lsb-u32"
 PALETTE_LUT_LAYOUT = "output-group-by-palette-lut"
 INT4_LAYOUT = "output-by-k-int4-lsb-u32"
 INT4_TILE_LAYOUT = "n16-k128-lane-major-int4-u32"
-INT4_SCALE_LAYOUT = "k-group-by-output-scale"
+INT4_TILE_SCALE_LAYOUT = "n16-k-group-major-scale"
 TILE_INNER = 32
 
 

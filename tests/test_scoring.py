@@ -156,7 +156,7 @@ def test_int4_dispatch_refuses(pk):
 
     def weight(**kw):
         w = dict(inner=128, columns=16, group=64, codes=K.GpuTensor("c", "uint32", (128, 16), rp.INT4_TILE_LAYOUT, t),
-                 scales=K.GpuTensor("s", "float16", (2, 16), rp.INT4_SCALE_LAYOUT, t))
+                 scales=K.GpuTensor("s", "float16", (2, 16), rp.INT4_TILE_SCALE_LAYOUT, t))
         return K.Int4Weight(**{**w, **kw})
 
     k = K.Int4GemvKernel.create(_FakeDevice())
@@ -165,7 +165,7 @@ def test_int4_dispatch_refuses(pk):
         k.create_dispatch({**base, "rows": 65})
     for change, match in ((dict(weight=t), "weight format"), (dict(activation="gelu"), "activation"),
                           (dict(weight=weight(codes=K.GpuTensor("c", "uint32", (128, 16), rp.INT4_LAYOUT, t))), "format"),
-                          (dict(weight=weight(scales=K.GpuTensor("s", "float32", (2, 16), rp.INT4_SCALE_LAYOUT,
+                          (dict(weight=weight(scales=K.GpuTensor("s", "float32", (2, 16), rp.INT4_TILE_SCALE_LAYOUT,
                                                                  t.float()))), "scales must be"),
                           (dict(bias=t, residual=t), "bias and residual"),
                           (dict(residual_scale=0.5), "residual scale without")):
