@@ -37,6 +37,9 @@
 // distributed shared memory.  Parts join in a fixed order: no workspace, no
 // atomics.
 #include <algorithm>
+#include <map>
+#include <mutex>
+#include <utility>
 
 #include "pk_common.cuh"
 #include "pk_internal.h"
@@ -51,7 +54,7 @@ constexpr int I4_SMEM = 220 * 1024;
 
 // Warps per CTA (registers: 72, 96, 128 a thread) and tiles in flight per warp.
 __host__ __device__ constexpr int i4_warps(int nt) { return nt == 1 ? 28 : nt == 2 ? 20 : 16; }
-__host__ __device__ constexpr int i4_depth(int gb) { return gb < 4 ? 2 : 3; }
+constexpr int I4_DEPTH = 3;
 
 struct I4Params {
   const void* a;
@@ -99,10 +102,10 @@ __device__ __forceinline__ void i4_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
 
 // D = A B + C: the first product of a group's sum.
 __device__ __forceinline__ void i4_mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1, float4 c) {
+                                             uint32_t b0, uint32_t b1, uint4 c) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(__uint_as_float(c.x)), "f"(__uint_as_float(c.y)), "f"(__uint_as_float(c.z)), "f"(__uint_as_float(c.w)));
 }
 
 __device__ __forceinline__ uint4 i4_load(const uint4* p) {
@@ -110,6 +113,17 @@ __device__ __forceinline__ uint4 i4_load(const uint4* p) {
   asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
       : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ uint4 i4_lds(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float i4_lds_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
   return v;
 }
 
@@ -132,70 +146,82 @@ __device__ __forceinline__ void i4_stage(const I4Params& p, unsigned char* xs, f
                                          int rows, int kt0, int tiles) {
   constexpr int PARTS = sizeof(T) == 2 ? 1 : 2;
   constexpr int SPT = 4 / GB;
+  constexpr int AHEAD = NT == 1 ? 2 : 4;  // loads in flight per lane: the rows come from L2 or beyond
   const int lane16 = threadIdx.x & 15;
-  const int jobs = rows * tiles;
+  const uint32_t mask = 0xffffu << (threadIdx.x & 16);  // this half of the warp
   const int stride = i4_col_bytes(p.ktiles_cta);
-  const int halves = (blockDim.x >> 5) * 2;  // half warps of the CTA
-  for (int j0 = (threadIdx.x >> 5) * 2; j0 < jobs; j0 += halves) {
-    const int j = min(j0 + (int)((threadIdx.x >> 4) & 1), jobs - 1);
-    const bool mine = j0 + (int)((threadIdx.x >> 4) & 1) < jobs;
-    const int r = j / tiles, kt = j % tiles;
+  // A half warp keeps its tile and walks the rows (or, with more tiles than
+  // half warps, walks the tiles too).
+  const int halves = blockDim.x >> 4, half = threadIdx.x >> 4;
+  const int side = max(1, halves / max(tiles, 1));  // half warps per tile
+  for (int kt = tiles <= halves ? (half < side * tiles ? half % max(tiles, 1) : tiles) : half; kt < tiles; kt += halves) {
     const int k = (kt0 + kt) * I4_KT + 8 * lane16;
-    const T* src = static_cast<const T*>(p.a) + (size_t)(row0 + r) * p.inner + k;
     const bool in = k < p.inner;  // inner is a multiple of 32: eight at once
-    uint4 col[PARTS];
-    if constexpr (PARTS == 1) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (in) v = *reinterpret_cast<const uint4*>(src);
-      col[0] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                          __byte_perm(v.y, v.w, 0x7632));
-    } else {
-      float v[8] = {};
-      if (in) {
-        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-        *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(src + 4);
-      }
-      uint32_t top = 0;
+    const T* src = static_cast<const T*>(p.a) + (size_t)row0 * p.inner + k;
+    for (int r0 = tiles <= halves ? half / tiles : 0; r0 < rows; r0 += side * AHEAD) {
+      uint4 raw[AHEAD][PARTS];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+      for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      // 2^s with the largest magnitude in [2^14, 2^15); s <= 126 keeps 2^s and 2^-s normal.
-      const int s = min(141 - (int)(top >> 23), 126);
-      const float up = __uint_as_float((uint32_t)(s + 127) << 23), down = __uint_as_float((uint32_t)(127 - s) << 23);
-      __half hi[8], lo[8];
+        for (int q = 0; q < PARTS; ++q)
+          raw[u][q] = in && r0 + u * side < rows ? reinterpret_cast<const uint4*>(src + (size_t)(r0 + u * side) * p.inner)[q]
+                                                 : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float y = v[i] * up;
-        hi[i] = __float2half_rn(y);
-        const float h = __half2float(hi[i]);
-        // An infinite or NaN input stands in the first column alone.
-        lo[i] = __float2half_rn(fabsf(h) <= 65504.0f ? y - h : 0.0f);
-      }
-      const int at[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-      __half* ha = reinterpret_cast<__half*>(&col[0]);
-      __half* hb = reinterpret_cast<__half*>(&col[PARTS - 1]);
+      for (int u = 0; u < AHEAD; ++u) {
+        const int r = r0 + u * side;
+        if (r >= rows) break;
+        uint4 col[PARTS];
+        if constexpr (PARTS == 1) {
+          const uint4 v = raw[u][0];
+          col[0] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                              __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+        } else {
+          float v[8];
+          *reinterpret_cast<uint4*>(v) = raw[u][0];
+          *reinterpret_cast<uint4*>(v + 4) = raw[u][PARTS - 1];
+          uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        ha[i] = hi[at[i]];
-        hb[i] = lo[at[i]];
-      }
-      if (mine && lane16 == 0) xscale[r * p.ktiles_cta + kt] = down;
-    }
+          for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
 #pragma unroll
-    for (int q = 0; q < PARTS; ++q) {
-      if (mine) *reinterpret_cast<uint4*>(xs + (size_t)(r * PARTS + q) * stride + kt * (I4_KT * 2) + lane16 * 16) = col[q];
-      // The second and fourth pairs of the eight; four lanes hold 32 inputs.
-      const float2 b = __half22float2(i4_h2(col[q].y)), d = __half22float2(i4_h2(col[q].w));
-      float sum = (b.x + b.y) + (d.x + d.y);
+          for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
+          // 2^s with the largest magnitude in [2^14, 2^15); s <= 126 keeps 2^s and 2^-s normal.
+          const int s = min(141 - (int)(top >> 23), 126);
+          const float up = __uint_as_float((uint32_t)(s + 127) << 23), down = __uint_as_float((uint32_t)(127 - s) << 23);
+          __half hi[8], lo[8];
 #pragma unroll
-      for (int o = 1; o < 4 * GB; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (mine && lane16 % (4 * GB) == 0) {
-        float* dst = i4_addend<NT>(addend, kt * SPT + lane16 / (4 * GB), r * PARTS + q);
-        // An infinite sum would meet the products' infinities as a NaN; they need no addend.
-        const float v = fabsf(sum) <= 3.0e38f || sum != sum ? -72.0f * sum : 0.0f;
-        dst[0] = v;
-        dst[2] = v;
+          for (int i = 0; i < 8; ++i) {
+            const float y = v[i] * up;
+            hi[i] = __float2half_rn(y);
+            const float h = __half2float(hi[i]);
+            // An infinite or NaN input stands in the first column alone.
+            lo[i] = __float2half_rn(fabsf(h) <= 65504.0f ? y - h : 0.0f);
+          }
+          const int at[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+          __half* ha = reinterpret_cast<__half*>(&col[0]);
+          __half* hb = reinterpret_cast<__half*>(&col[PARTS - 1]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            ha[i] = hi[at[i]];
+            hb[i] = lo[at[i]];
+          }
+          if (lane16 == 0) xscale[r * p.ktiles_cta + kt] = down;
+        }
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+          *reinterpret_cast<uint4*>(xs + (size_t)(r * PARTS + q) * stride + kt * (I4_KT * 2) + lane16 * 16) = col[q];
+          // The second and fourth pairs of the eight; four lanes hold 32 inputs.
+          const float2 b = __half22float2(i4_h2(col[q].y)), d = __half22float2(i4_h2(col[q].w));
+          float sum = (b.x + b.y) + (d.x + d.y);
+#pragma unroll
+          for (int o = 1; o < 4 * GB; o <<= 1) sum += __shfl_xor_sync(mask, sum, o);
+          if (lane16 % (4 * GB) == 0) {
+            float* dst = i4_addend<NT>(addend, kt * SPT + lane16 / (4 * GB), r * PARTS + q);
+            // An infinite sum would meet the products' infinities as a NaN; they need no addend.
+            const float v = fabsf(sum) <= 3.0e38f || sum != sum ? -72.0f * sum : 0.0f;
+            dst[0] = v;
+            dst[2] = v;
+          }
+        }
       }
     }
   }
@@ -208,8 +234,9 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
   extern __shared__ __align__(128) unsigned char i4_smem[];
   constexpr int PARTS = sizeof(T) == 2 ? 1 : 2;  // columns per row
   constexpr int SPT = 4 / GB;                    // scales per tile and output
-  constexpr int DEPTH = i4_depth(GB);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int DEPTH = I4_DEPTH;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // the same in all lanes, and known to be
   const int g = lane >> 2, t = lane & 3;
   const int wm = warp / p.wk, wk = warp % p.wk;
   const int rank = p.cluster > 1 ? (int)cluster_ctarank() : 0;
@@ -227,7 +254,7 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
 
   struct Slot {
     uint4 code[2];
-    T scale[2][SPT];
+    T scale[2];  // of the tile's scale t % SPT; lanes exchange them when they are used
   };
   Slot ring[DEPTH];
   // What is loaded next: this warp's tile `lk` of inputs (of the CTA's) for
@@ -249,12 +276,10 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
       s.code[0] = i4_load(lcode);
       s.code[1] = i4_load(lcode + 32);
       const int kt = k0 + lk;
-#pragma unroll
-      for (int b = 0; b < SPT; ++b) {
-        const int gi = GB == 4 ? (p.group_inv ? (int)__umulhi((uint32_t)kt, p.group_inv) : kt) : min(kt * SPT + b, p.groups - 1);
-        s.scale[0][b] = __ldg(lscale + gi * 16);
-        s.scale[1][b] = __ldg(lscale + gi * 16 + 8);
-      }
+      const int gi = GB == 4 ? (p.group_inv ? (int)__umulhi((uint32_t)kt, p.group_inv) : kt)
+                             : min(kt * SPT + (t & (SPT - 1)), p.groups - 1);
+      s.scale[0] = __ldg(lscale + gi * 16);
+      s.scale[1] = __ldg(lscale + gi * 16 + 8);
     }
     lk += p.wk;
     lcode += p.wk * 64;
@@ -273,13 +298,13 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
   i4_stage<T, NT, GB>(p, xs, xscale, addend, row0, rows, k0, ktiles);
   __syncthreads();
 
-  const unsigned char* xcol[NT];
-  const float* xsc[NT];
+  uint32_t xcol[NT], xsc[NT];  // shared memory addresses
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    xcol[n] = xs + (size_t)min(n * 8 + g, cols - 1) * stride + t * 16;
-    xsc[n] = xscale + min(n * 4 + t, rows - 1) * p.ktiles_cta;  // FP32: columns 2 t and 2 t + 1 are one row
+    xcol[n] = smem_addr(xs + (size_t)min(n * 8 + g, cols - 1) * stride + t * 16);
+    xsc[n] = smem_addr(xscale + min(n * 4 + t, rows - 1) * p.ktiles_cta);  // FP32: columns 2 t and 2 t + 1 are one row
   }
+  const uint32_t xadd = smem_addr(addend) + t * 16;
   const int M = p.wm * 16;
   constexpr int PC = NT * 8;
   float* part = reinterpret_cast<float*>(i4_smem + p.part_offset);  // [wk][column][output]
@@ -302,7 +327,7 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
               uint4 x[NT];
 #pragma unroll
               for (int n = 0; n < NT; ++n)
-                x[n] = *reinterpret_cast<const uint4*>(xcol[n] + kl * (I4_KT * 2) + i * 64);
+                x[n] = i4_lds(xcol[n] + kl * (I4_KT * 2) + i * 64);
               uint32_t w0[4], w1[4];
               i4_expand((&s.code[0].x)[i], w0);
               i4_expand((&s.code[1].x)[i], w1);
@@ -310,18 +335,22 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
               for (int n = 0; n < NT; ++n) {
                 if (i == b * GB)
                   i4_mma_first(acc[n], w0[0], w1[0], w0[1], w1[1], x[n].x, x[n].y,
-                               *reinterpret_cast<const float4*>(addend + (size_t)((kl * SPT + b) * NT * 4 + n * 4 + t) * 4));
+                               i4_lds(xadd + (kl * SPT + b) * (NT * 64) + n * 64));
                 else
                   i4_mma(acc[n], w0[0], w1[0], w0[1], w1[1], x[n].x, x[n].y);
                 i4_mma(acc[n], w0[2], w1[2], w0[3], w1[3], x[n].z, x[n].w);
               }
             }
-            const float s0 = (float)s.scale[0][b], s1 = (float)s.scale[1][b];
+            float s0 = (float)s.scale[0], s1 = (float)s.scale[1];
+            if constexpr (SPT > 1) {
+              s0 = __shfl_sync(0xffffffffu, s0, (lane & ~3) | b);
+              s1 = __shfl_sync(0xffffffffu, s1, (lane & ~3) | b);
+            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               float f0 = s0, f1 = s1;
               if constexpr (PARTS == 2) {
-                const float f = xsc[n][kl];
+                const float f = i4_lds_f32(xsc[n] + 4 * kl);
                 f0 *= f;
                 f1 *= f;
               }
@@ -385,6 +414,41 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
   }
 }
 
+// Clusters of `cluster` CTAs that run at once with one CTA per SM (fewer than
+// SMs / cluster: a cluster stays within a GPC, and GPCs differ in size).
+int i4_clusters(const DeviceCtx& dev, int cluster, int* out) {
+  if (cluster == 1) {
+    *out = dev.sm_count;
+    return PK_OK;
+  }
+  static std::mutex mu;
+  static std::map<std::pair<int, int>, int> known;
+  std::lock_guard<std::mutex> lock(mu);
+  int& n = known[{dev.ordinal, cluster}];
+  if (n == 0) {
+    const void* kernel = reinterpret_cast<const void*>(int4_gemv_kernel<__half, 1, 4>);
+    const int st = set_max_dynamic_smem(kernel, I4_SMEM);
+    if (st != PK_OK) return st;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)cluster;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)cluster);
+    cfg.blockDim = dim3(i4_warps(1) * 32);
+    cfg.dynamicSmemBytes = I4_SMEM;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int most = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&most, kernel, &cfg);
+    if (e != cudaSuccess) return cuda_error(e, "occupancy query (int4 product)");
+    n = std::max(1, most);
+  }
+  *out = n;
+  return PK_OK;
+}
+
 template <typename T, int NT, int GB>
 int launch_one(const I4Params& p, dim3 grid, int smem, cudaStream_t stream) {
   const void* kernel = reinterpret_cast<const void*>(int4_gemv_kernel<T, NT, GB>);
@@ -419,7 +483,7 @@ int launch_typed(const DeviceCtx& dev, I4Params p, int group, cudaStream_t strea
   constexpr int PARTS = sizeof(T) == 2 ? 1 : 2;
   const int mtiles = (p.columns + 15) / 16;
   int cols = std::min(p.rows * PARTS, I4_COLS);
-  int nt = 0, smem = 0;
+  int nt = 0, smem = 0, clusters = 0;
   // Columns per pass, then CTAs per cluster: the least that fit.
   for (;; cols = std::max(PARTS, cols / 2 / PARTS * PARTS)) {
     p.rows_per_pass = cols / PARTS;
@@ -429,7 +493,8 @@ int launch_typed(const DeviceCtx& dev, I4Params p, int group, cudaStream_t strea
       // Few outputs: the inputs over more SMs, while each has a tile for every warp of 4.
       if (mtiles * p.cluster * 2 <= dev.sm_count && p.cluster < I4_CLUSTER && p.ktiles >= p.cluster * 2 * 4) continue;
       p.ktiles_cta = (p.ktiles + p.cluster - 1) / p.cluster;
-      const int clusters = dev.sm_count / p.cluster;
+      const int st = i4_clusters(dev, p.cluster, &clusters);
+      if (st != PK_OK) return st;
       const int q = (mtiles + clusters - 1) / clusters;  // output tiles of a cluster
       const int turns = (q + warps - 1) / warps;
       p.wm = (q + turns - 1) / turns;
@@ -444,7 +509,7 @@ int launch_typed(const DeviceCtx& dev, I4Params p, int group, cudaStream_t strea
   }
   if (smem > I4_SMEM) return set_error(PK_E_SHAPE, "int4 products of K=%d do not fit shared memory", p.inner);
   const int passes = (p.rows + p.rows_per_pass - 1) / p.rows_per_pass;
-  const int clusters = std::min(dev.sm_count / p.cluster, (mtiles + p.wm - 1) / p.wm);
+  clusters = std::min(clusters, (mtiles + p.wm - 1) / p.wm);
   const dim3 grid((unsigned)(clusters * p.cluster), (unsigned)passes);
   if (nt == 1) return launch_group<T, 1>(p, group, grid, smem, stream);
   if (nt == 2) return launch_group<T, 2>(p, group, grid, smem, stream);
