@@ -425,7 +425,7 @@ int pk_residual_norm(pk_device* device, const pk_residual_norm_desc* d, pk_strea
     }
   DeviceScope scope(device->ctx);
   if (scope.status != PK_OK) return scope.status;
-  return launch_residual_norm(*d, as_stream(stream));
+  return launch_residual_norm(device->ctx, *d, as_stream(stream));
 }
 
 int pk_int4_gemv(pk_device* device, const pk_int4_gemv_desc* d, pk_stream stream) {

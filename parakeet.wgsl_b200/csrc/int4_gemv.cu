@@ -146,7 +146,7 @@ __device__ __forceinline__ void i4_stage(const I4Params& p, unsigned char* xs, f
                                          int rows, int kt0, int tiles) {
   constexpr int PARTS = sizeof(T) == 2 ? 1 : 2;
   constexpr int SPT = 4 / GB;
-  constexpr int AHEAD = NT == 1 ? 2 : 4;  // loads in flight per lane: the rows come from L2 or beyond
+  constexpr int AHEAD = NT == 1 ? (PARTS == 1 ? 4 : 2) : 4;  // loads in flight per lane: the rows come from L2 or beyond
   const int lane16 = threadIdx.x & 15;
   const uint32_t mask = 0xffffu << (threadIdx.x & 16);  // this half of the warp
   const int stride = i4_col_bytes(p.ktiles_cta);

@@ -119,7 +119,7 @@ int launch_subsampling_time_mask(int precision, int batch, int height, int width
 
 // Scoring operators (token_scores.cu, residual_norm.cu, int4_gemv.cu, joint_logits.cu).
 int launch_token_scores(const DeviceCtx& dev, const pk_token_scores_desc& d, cudaStream_t stream);
-int launch_residual_norm(const pk_residual_norm_desc& d, cudaStream_t stream);
+int launch_residual_norm(const DeviceCtx& dev, const pk_residual_norm_desc& d, cudaStream_t stream);
 int launch_int4_gemv(const DeviceCtx& dev, const pk_int4_gemv_desc& d, cudaStream_t stream);
 int launch_joint_logits(const DeviceCtx& dev, const pk_joint_logits_desc& d, cudaStream_t stream);
 

@@ -15,6 +15,8 @@
 // between reaches memory.  A row lives in the registers of 32 to 1024 threads;
 // all its loads are issued before the first is used, and gamma, beta and gate
 // come from L1 after the first rows.
+#include <algorithm>
+
 #include "pk_common.cuh"
 #include "pk_internal.h"
 
@@ -67,9 +69,15 @@ __device__ __forceinline__ void rn_unpack(const typename RnWord<VEC * sizeof(T)>
 template <typename T, int VEC>
 __device__ __forceinline__ typename RnWord<VEC * sizeof(T)>::type rn_pack(const float (&v)[VEC]) {
   typename RnWord<VEC * sizeof(T)>::type raw;
-  T* e = reinterpret_cast<T*>(&raw);
+  if constexpr (sizeof(T) == 2 && VEC > 1) {
+    __half2* e2 = reinterpret_cast<__half2*>(&raw);
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) e[j] = (T)v[j];
+    for (int j = 0; j < VEC / 2; ++j) e2[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+  } else {
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) e[j] = (T)v[j];
+  }
   return raw;
 }
 template <int VEC>
@@ -81,6 +89,12 @@ __device__ __forceinline__ void rn_params(const float* src, float (&v)[VEC]) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) v[j] = __ldg(src + j);
   }
+}
+
+// 1 / sqrt(v): the hardware's estimate (2 ulp) and one Newton step.
+__device__ __forceinline__ float rn_rsqrt(float v) {
+  const float r = rsqrtf(v);
+  return fmaf(r * 0.5f, fmaf(-v * r, r, 1.0f), r);
 }
 
 // Sum over the G threads of a row.  Rows of more than a warp meet in shared
@@ -162,7 +176,7 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) residual_norm_kernel(const 
         }
       }
     }
-    rstd = 1.0f / sqrtf(rn_sum<G>(s, red, turn) * inv + p.eps);
+    rstd = rn_rsqrt(rn_sum<G>(s, red, turn) * inv + p.eps);
   };
   float mean = 0.0f, rstd = 1.0f;
   if (p.post != PK_NORM_NONE) stats(p.post, mean, rstd);
@@ -220,6 +234,194 @@ __global__ void __launch_bounds__(G > 256 ? G : 256) residual_norm_kernel(const 
   }
 }
 
+// Many rows of at most 512 vectors: a thread keeps one vector of channels for
+// every row that its CTA takes, so the parameters stay in its registers (a gate
+// that all rows share folded with the scale into gamma and beta), and the CTA
+// takes R rows at a time: their sums meet at the same barriers, and the next R
+// rows are on their way meanwhile.
+constexpr int RN_R = 4;
+constexpr int RN_COLS = 512;  // threads per CTA, at most
+
+// Sums the CTA's R values per thread; all threads receive last(total) of each.  The
+// warp's butterfly halves what a lane holds as long as it holds more than one
+// value, so R sums cost R + 2 exchanges, not 5 R.  `turn` alternates two halves
+// of `red`: one barrier a sum is enough.
+template <typename Last>
+__device__ __forceinline__ void rn_sums(float (&v)[RN_R], float (*red)[RN_COLS / 32][RN_R], int& turn, Last last) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const bool b4 = lane & 16, b3 = lane & 8;
+  float k0 = b4 ? v[2] : v[0], k1 = b4 ? v[3] : v[1];
+  k0 += __shfl_xor_sync(0xffffffffu, b4 ? v[0] : v[2], 16);
+  k1 += __shfl_xor_sync(0xffffffffu, b4 ? v[1] : v[3], 16);
+  float k = b3 ? k1 : k0;
+  k += __shfl_xor_sync(0xffffffffu, b3 ? k0 : k1, 8);
+  k += __shfl_xor_sync(0xffffffffu, k, 4);
+  k += __shfl_xor_sync(0xffffffffu, k, 2);
+  k += __shfl_xor_sync(0xffffffffu, k, 1);
+  float(*mine)[RN_R] = red[turn];
+  turn ^= 1;
+  if ((lane & 7) == 0) mine[warp][lane >> 3] = k;
+  __syncthreads();
+  // Lane (w, r): the sums of row r in warps w, w + 8.
+  const int w = lane >> 2, r = lane & 3;
+  k = w < warps ? mine[w][r] : 0.0f;
+  if (w + 8 < warps) k += mine[w + 8][r];
+  k += __shfl_xor_sync(0xffffffffu, k, 4);
+  k += __shfl_xor_sync(0xffffffffu, k, 8);
+  k = last(k + __shfl_xor_sync(0xffffffffu, k, 16));
+#pragma unroll
+  for (int i = 0; i < RN_R; ++i) v[i] = __shfl_sync(0xffffffffu, k, i);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(RN_COLS, 1) residual_norm_rows_kernel(const RnParams p) {
+  pdl_entry();
+  constexpr int VEC = 16 / sizeof(T), P = VEC / 2;
+  __shared__ float red[2][RN_COLS / 32][RN_R];
+  const int C = p.channels;
+  const int c = threadIdx.x * VEC;
+  const bool in = c < C;  // the last warp may reach past the row
+  const bool by_rows = p.gate && p.gate_rows > 0;
+  const float2 one = make_float2(1.0f, 1.0f), zero = make_float2(0.0f, 0.0f);
+  uint4 fr[RN_R], xr[RN_R];
+  // Rows left from the batch's first, and its first element of this thread.
+  const int step = (int)gridDim.x * RN_R;
+  int left = (int)(p.rows - (int64_t)blockIdx.x * RN_R);
+  int64_t at = (int64_t)blockIdx.x * RN_R * C + c;
+  auto fetch = [&](int64_t from, int rows) {
+    const T* fp = static_cast<const T*>(p.f) + from;
+    const T* xp = static_cast<const T*>(p.x) + from;
+#pragma unroll
+    for (int i = 0; i < RN_R; ++i) {
+      const bool live = in && i < rows;
+      fr[i] = live ? *reinterpret_cast<const uint4*>(fp + (size_t)(uint32_t)(i * C)) : make_uint4(0u, 0u, 0u, 0u);
+      xr[i] = live ? *reinterpret_cast<const uint4*>(xp + (size_t)(uint32_t)(i * C)) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  fetch(at, left);
+  float2 sg[P], sb[P], hg[P], hb[P];  // post and pre gamma and beta
+#pragma unroll
+  for (int j = 0; j < P; ++j) sg[j] = hg[j] = one, sb[j] = hb[j] = zero;
+  if (in) {
+    auto take = [&](const float* src, float2 (&dst)[P]) {
+#pragma unroll
+      for (int j = 0; j < P; j += 2) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(src + c + 2 * j));
+        dst[j] = make_float2(v.x, v.y);
+        dst[j + 1] = make_float2(v.z, v.w);
+      }
+    };
+    if (p.post != PK_NORM_NONE) take(p.post_gamma, sg);
+    if (p.post == PK_NORM_LAYER) take(p.post_beta, sb);
+    if (p.pre != PK_NORM_NONE) take(p.pre_gamma, hg);
+    if (p.pre == PK_NORM_LAYER) take(p.pre_beta, hb);
+    if (!by_rows) {
+      float2 g[P];
+#pragma unroll
+      for (int j = 0; j < P; ++j) g[j] = one;
+      if (p.gate) take(p.gate, g);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        g[j] = make_float2(g[j].x * p.scale, g[j].y * p.scale);
+        sg[j] = ffma2(sg[j], g[j], zero);
+        sb[j] = ffma2(sb[j], g[j], zero);
+      }
+    }
+  }
+  const float inv = 1.0f / (float)C;
+  int turn = 0;
+  float2 v[RN_R][P];
+  float rstd[RN_R];
+  // Centres the rows in v (LayerNorm) and sets rstd = 1 / deviation; threads
+  // past the row hold zeros.
+  auto normalize = [&](int kind) {
+    float s[RN_R];
+    if (kind == PK_NORM_LAYER) {
+#pragma unroll
+      for (int i = 0; i < RN_R; ++i) {
+        float2 a = v[i][0];
+#pragma unroll
+        for (int j = 1; j < P; ++j) a = ffma2(v[i][j], one, a);
+        s[i] = a.x + a.y;
+      }
+      rn_sums(s, red, turn, [&](float k) { return -k * inv; });
+#pragma unroll
+      for (int i = 0; i < RN_R; ++i) {
+        const float m = in ? s[i] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < P; ++j) v[i][j] = ffma2(v[i][j], one, make_float2(m, m));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < RN_R; ++i) {
+      float2 a = ffma2(v[i][0], v[i][0], zero);
+#pragma unroll
+      for (int j = 1; j < P; ++j) a = ffma2(v[i][j], v[i][j], a);
+      s[i] = a.x + a.y;
+    }
+    rn_sums(s, red, turn, [&](float k) { return rn_rsqrt(fmaf(k, inv, p.eps)); });
+#pragma unroll
+    for (int i = 0; i < RN_R; ++i) rstd[i] = s[i];
+  };
+  for (; left > 0; left -= step, at += (int64_t)step * C) {
+#pragma unroll
+    for (int i = 0; i < RN_R; ++i) {
+      float e[VEC];
+      rn_unpack<T, VEC>(fr[i], e);
+#pragma unroll
+      for (int j = 0; j < P; ++j) v[i][j] = make_float2(e[2 * j], e[2 * j + 1]);
+      rstd[i] = 1.0f;
+    }
+    uint4 xc[RN_R];
+#pragma unroll
+    for (int i = 0; i < RN_R; ++i) xc[i] = xr[i];
+    if (left > step) fetch(at + (int64_t)step * C, left - step);
+    if (p.post != PK_NORM_NONE) normalize(p.post);
+#pragma unroll
+    for (int i = 0; i < RN_R; ++i) {
+      float e[VEC], y[VEC];
+      rn_unpack<T, VEC>(xc[i], e);
+      float2 w[P];
+#pragma unroll
+      for (int j = 0; j < P; ++j) w[j] = one;
+      if (by_rows && in && i < left) {
+        const float* gate = p.gate + (p.rows - left + i) / p.gate_rows * C + c;
+#pragma unroll
+        for (int j = 0; j < P; j += 2) {
+          const float4 g = __ldg(reinterpret_cast<const float4*>(gate + 2 * j));
+          w[j] = make_float2(g.x * p.scale, g.y * p.scale);
+          w[j + 1] = make_float2(g.z * p.scale, g.w * p.scale);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        float2 u = ffma2(v[i][j], make_float2(rstd[i], rstd[i]), zero);
+        u = ffma2(u, sg[j], sb[j]);
+        u = ffma2(u, w[j], make_float2(e[2 * j], e[2 * j + 1]));
+        v[i][j] = u;
+        y[2 * j] = u.x;
+        y[2 * j + 1] = u.y;
+      }
+      if (in && i < left)
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.y) + at + (size_t)(uint32_t)(i * C)) = rn_pack<T, VEC>(y);
+    }
+    if (p.pre == PK_NORM_NONE) continue;
+    normalize(p.pre);
+#pragma unroll
+    for (int i = 0; i < RN_R; ++i) {
+      float h[VEC];
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const float2 u = ffma2(ffma2(v[i][j], make_float2(rstd[i], rstd[i]), zero), hg[j], hb[j]);
+        h[2 * j] = u.x;
+        h[2 * j + 1] = u.y;
+      }
+      if (in && i < left)
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.h) + at + (size_t)(uint32_t)(i * C)) = rn_pack<T, VEC>(h);
+    }
+  }
+}
+
 template <typename T, int VEC, int G, int NV>
 int launch_one(const RnParams& p, cudaStream_t stream) {
   constexpr int threads = G > 256 ? G : 256;
@@ -248,21 +450,34 @@ int launch_vec(const RnParams& p, cudaStream_t stream) {
 }
 
 template <typename T>
-int launch_typed(const RnParams& p, cudaStream_t stream) {
+int launch_rows(const DeviceCtx& dev, const RnParams& p, cudaStream_t stream) {
+  const int threads = (p.channels * (int)sizeof(T) / 16 + 31) / 32 * 32;
+  const int64_t ctas = std::min<int64_t>((p.rows + RN_R - 1) / RN_R, (int64_t)dev.sm_count * (RN_COLS / threads));
+  return cuda_error(launch_kernel(residual_norm_rows_kernel<T>, dim3((unsigned)ctas), dim3((unsigned)threads), 0, stream, p),
+                    "residual_norm launch");
+}
+
+template <typename T>
+int launch_typed(const DeviceCtx& dev, const RnParams& p, cudaStream_t stream) {
   const uintptr_t data = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.f) |
                          reinterpret_cast<uintptr_t>(p.y) | reinterpret_cast<uintptr_t>(p.h) |
                          (uintptr_t)p.channels * sizeof(T);
   const uintptr_t params = reinterpret_cast<uintptr_t>(p.post_gamma) | reinterpret_cast<uintptr_t>(p.post_beta) |
                            reinterpret_cast<uintptr_t>(p.pre_gamma) | reinterpret_cast<uintptr_t>(p.pre_beta) |
                            reinterpret_cast<uintptr_t>(p.gate);
-  if ((data & 15) == 0 && (params & 15) == 0) return launch_vec<T, 16 / sizeof(T)>(p, stream);
+  if ((data & 15) == 0 && (params & 15) == 0) {
+    const int64_t vectors = p.channels * (int64_t)sizeof(T) / 16;
+    // Enough rows for every SM to take several.
+    if (vectors <= RN_COLS && p.rows * vectors >= (int64_t)RN_R * RN_COLS * dev.sm_count / 2) return launch_rows<T>(dev, p, stream);
+    return launch_vec<T, 16 / sizeof(T)>(p, stream);
+  }
   if (sizeof(T) == 2 && (data & 7) == 0 && (params & 15) == 0) return launch_vec<T, 8 / sizeof(T)>(p, stream);
   return launch_vec<T, 1>(p, stream);
 }
 
 }  // namespace
 
-int launch_residual_norm(const pk_residual_norm_desc& d, cudaStream_t stream) {
+int launch_residual_norm(const DeviceCtx& dev, const pk_residual_norm_desc& d, cudaStream_t stream) {
   RnParams p;
   p.x = d.input;
   p.f = d.block;
@@ -280,7 +495,7 @@ int launch_residual_norm(const pk_residual_norm_desc& d, cudaStream_t stream) {
   p.pre = d.pre;
   p.scale = d.residual_scale;
   p.eps = d.epsilon;
-  return d.precision == PK_FP16 ? launch_typed<__half>(p, stream) : launch_typed<float>(p, stream);
+  return d.precision == PK_FP16 ? launch_typed<__half>(dev, p, stream) : launch_typed<float>(dev, p, stream);
 }
 
 }  // namespace pk

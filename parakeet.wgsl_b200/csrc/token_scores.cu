@@ -117,6 +117,14 @@ __device__ __forceinline__ void ts_shift(float g, float& s, float& u) {
   u = c == 0.0f ? 0.0f : c * fmaf(g, s, u);  // once 2^g is 0 nothing is left
   s *= c;
 }
+// The same of a pair of sums.
+__device__ __forceinline__ void ts_shift(float g, float2& s, float2& u) {
+  const float c = ts_ex2(g);
+  const float d = c == 0.0f ? 0.0f : g;
+  const float2 c2 = make_float2(c, c), zero = make_float2(0.0f, 0.0f);
+  u = ffma2(ffma2(s, make_float2(d, d), u), c2, zero);
+  s = ffma2(s, c2, zero);
+}
 __device__ __forceinline__ TsStat ts_join(TsStat a, TsStat b) {
   TsStat r{fmaxf(a.m, b.m), 0.0f, 0.0f};
   auto add = [&](TsStat p) {
@@ -196,9 +204,9 @@ struct TsTile {
     }
   }
   __device__ __forceinline__ float maximum() const { return largest(raw, N); }
-  // s += sum 2^t, u += sum 2^t t for t = x ts_factor(m) - ts_base(m).
-  __device__ __forceinline__ void sums(float m, float2& s, float2& u) const {
-    const float a = ts_factor(m), b = -ts_base(m);
+  // s += sum 2^t, u += sum 2^t t for t = x a - base (of the maximum m).
+  __device__ __forceinline__ void sums(float m, float a, float base, float2& s, float2& u) const {
+    const float b = -base;
     const float2 a2 = make_float2(a, a), b2 = make_float2(b, b), one = make_float2(1.0f, 1.0f);
     auto add = [&](float2 t) {
       const float2 e = make_float2(ts_ex2(t.x), ts_ex2(t.y));
@@ -380,7 +388,7 @@ __global__ void __launch_bounds__(TS_THREADS, sizeof(T) == 2 && NV > 0 ? (NV == 
     const float mine = tile.maximum();
     st.m = ts_value(__reduce_max_sync(0xffffffffu, ts_ordered(mine)));
     float2 s2 = make_float2(0.0f, 0.0f), u2 = make_float2(0.0f, 0.0f);
-    tile.sums(st.m, s2, u2);
+    tile.sums(st.m, ts_factor(st.m), ts_base(st.m), s2, u2);
     st.s = s2.x + s2.y;
     st.u = u2.x + u2.y;
 #pragma unroll
@@ -428,18 +436,17 @@ __global__ void __launch_bounds__(TS_THREADS, sizeof(T) == 2 && NV > 0 ? (NV == 
   } else {
     const int step = warps * 32 * TS_UNR, first = gw * 32 * TS_UNR;
     float2 s2 = make_float2(0.0f, 0.0f), u2 = make_float2(0.0f, 0.0f);
-    float m = -INFINITY;
+    float m = -INFINITY, ma = TS_LOG2E, mb = 0.0f;  // the maximum, its factor and base
     auto take = [&](const TsTile<T, TS_UNR>& tile) {
       const float tm = tile.maximum();
       if (tm > m) {
-        if (m > -INFINITY) {
-          const float g = ts_base(m) - ts_base(tm);
-          ts_shift(g, s2.x, u2.x);
-          ts_shift(g, s2.y, u2.y);
-        }
+        const float to = ts_base(tm);
+        if (m > -INFINITY) ts_shift(mb - to, s2, u2);
         m = tm;
+        ma = ts_factor(tm);
+        mb = to;
       }
-      tile.sums(m, s2, u2);
+      tile.sums(m, ma, mb, s2, u2);
     };
     // The next tile is on its way while one is summed.
     TsTile<T, TS_UNR> a, b;
@@ -451,13 +458,13 @@ __global__ void __launch_bounds__(TS_THREADS, sizeof(T) == 2 && NV > 0 ? (NV == 
       if (v + 2 * step < vectors) a.load(base, skew, columns, v + 2 * step, lane, 32, vectors);
       take(b);
     }
-    st = TsStat{m, s2.x + s2.y, u2.x + u2.y};
+    // The lanes' sums, brought to the warp's maximum.
+    st = TsStat{ts_value(__reduce_max_sync(0xffffffffu, ts_ordered(m))), s2.x + s2.y, u2.x + u2.y};
+    if (st.s != 0.0f && m != st.m) ts_shift(mb - ts_base(st.m), st.s, st.u);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      const TsStat other{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                         __shfl_xor_sync(0xffffffffu, st.u, o)};
-      // Both lanes of a pair join in the same order.
-      st = (lane & o) ? ts_join(other, st) : ts_join(st, other);
+      st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
+      st.u += __shfl_xor_sync(0xffffffffu, st.u, o);
     }
     if (k > 0) {
       const float bound = ts_value(ts_bound(sm, ts_ordered(m), group, wpr, k));

@@ -308,7 +308,8 @@ def _rows(rng, rows, channels, profile, std=1.0, mean=0.0):
 
 @pytest.mark.parametrize("profile", ["fp16", "fp32"])
 @pytest.mark.parametrize("rows,channels", [(1, 4), (1, 640), (9, 1024), (3, 68), (2, 1500), (5, 2048), (3, 4100), (2, 8192),
-                                           (1, 16388), (2, 32768), (1000, 64)])
+                                           (1, 16388), (2, 32768), (1000, 64), (2401, 640), (5003, 264), (2370, 1024),
+                                           (1201, 2048), (20001, 16)])
 def test_residual_norm_shapes(pk, device, profile, rows, channels):
     rng = np.random.default_rng(rows + channels)
     x, f = _rows(rng, rows, channels, profile, 2.0), _rows(rng, rows, channels, profile, 1.5, 0.3)
@@ -320,21 +321,22 @@ def test_residual_norm_shapes(pk, device, profile, rows, channels):
 @pytest.mark.parametrize("post", ["none", "layer", "rms"])
 @pytest.mark.parametrize("pre", ["none", "layer", "rms"])
 @pytest.mark.parametrize("gate_rows", [None, 0, 3, 7])
-def test_residual_norm_kinds_and_gates(pk, device, profile, post, pre, gate_rows):
+@pytest.mark.parametrize("rows", [13, 4099])
+def test_residual_norm_kinds_and_gates(pk, device, profile, post, pre, gate_rows, rows):
     rng = np.random.default_rng(11)
-    x, f = _rows(rng, 13, 320, profile, 2.0), _rows(rng, 13, 320, profile)
+    x, f = _rows(rng, rows, 320, profile, 2.0), _rows(rng, rows, 320, profile)
     gate = None
     if gate_rows is not None:
-        gate = rng.standard_normal((1 if gate_rows == 0 else -(-13 // gate_rows), 320)).astype(np.float32)
+        gate = rng.standard_normal((1 if gate_rows == 0 else -(-rows // gate_rows), 320)).astype(np.float32)
     _residual_norm(pk, device, x, f, profile, post, pre, gate, gate_rows or 0, scale=0.25)
 
 
 @pytest.mark.parametrize("place", ["input", "both", "swapped"])
 @pytest.mark.parametrize("pre", ["none", "layer"])
-@pytest.mark.parametrize("channels", [640, 4096])
-def test_residual_norm_in_place(pk, device, place, pre, channels):
+@pytest.mark.parametrize("rows,channels", [(11, 640), (11, 4096), (2500, 640)])
+def test_residual_norm_in_place(pk, device, place, pre, rows, channels):
     rng = np.random.default_rng(12)
-    x, f = _rows(rng, 11, channels, "fp16", 2.0), _rows(rng, 11, channels, "fp16")
+    x, f = _rows(rng, rows, channels, "fp16", 2.0), _rows(rng, rows, channels, "fp16")
     want = _residual_norm(pk, device, x, f, "fp16", "layer", pre, scale=0.5)
     got = _residual_norm(pk, device, x, f, "fp16", "layer", pre, scale=0.5, place=place)
     np.testing.assert_array_equal(got[0], want[0])
