@@ -273,7 +273,7 @@ __device__ __forceinline__ void rn_sums(float (&v)[RN_R], float (*red)[RN_COLS /
   for (int i = 0; i < RN_R; ++i) v[i] = __shfl_sync(0xffffffffu, k, i);
 }
 
-template <typename T>
+template <typename T, bool BY_ROWS>
 __global__ void __launch_bounds__(RN_COLS, 1) residual_norm_rows_kernel(const RnParams p) {
   pdl_entry();
   constexpr int VEC = 16 / sizeof(T), P = VEC / 2;
@@ -281,24 +281,21 @@ __global__ void __launch_bounds__(RN_COLS, 1) residual_norm_rows_kernel(const Rn
   const int C = p.channels;
   const int c = threadIdx.x * VEC;
   const bool in = c < C;  // the last warp may reach past the row
-  const bool by_rows = p.gate && p.gate_rows > 0;
+  const uint32_t gate_rows = (uint32_t)min(p.gate_rows, p.rows);  // rows are below 2^31
   const float2 one = make_float2(1.0f, 1.0f), zero = make_float2(0.0f, 0.0f);
   uint4 fr[RN_R], xr[RN_R];
   // Rows left from the batch's first, and its first element of this thread.
   const int step = (int)gridDim.x * RN_R;
   int left = (int)(p.rows - (int64_t)blockIdx.x * RN_R);
   int64_t at = (int64_t)blockIdx.x * RN_R * C + c;
-  auto fetch = [&](int64_t from, int rows) {
-    const T* fp = static_cast<const T*>(p.f) + from;
-    const T* xp = static_cast<const T*>(p.x) + from;
+  auto fetch = [&](const void* src, int64_t from, int rows, uint4 (&raw)[RN_R]) {
+    const T* s = static_cast<const T*>(src) + from;
 #pragma unroll
-    for (int i = 0; i < RN_R; ++i) {
-      const bool live = in && i < rows;
-      fr[i] = live ? *reinterpret_cast<const uint4*>(fp + (size_t)(uint32_t)(i * C)) : make_uint4(0u, 0u, 0u, 0u);
-      xr[i] = live ? *reinterpret_cast<const uint4*>(xp + (size_t)(uint32_t)(i * C)) : make_uint4(0u, 0u, 0u, 0u);
-    }
+    for (int i = 0; i < RN_R; ++i)
+      raw[i] = in && i < rows ? *reinterpret_cast<const uint4*>(s + (size_t)(uint32_t)(i * C)) : make_uint4(0u, 0u, 0u, 0u);
   };
-  fetch(at, left);
+  fetch(p.f, at, left, fr);
+  fetch(p.x, at, left, xr);
   float2 sg[P], sb[P], hg[P], hb[P];  // post and pre gamma and beta
 #pragma unroll
   for (int j = 0; j < P; ++j) sg[j] = hg[j] = one, sb[j] = hb[j] = zero;
@@ -315,7 +312,7 @@ __global__ void __launch_bounds__(RN_COLS, 1) residual_norm_rows_kernel(const Rn
     if (p.post == PK_NORM_LAYER) take(p.post_beta, sb);
     if (p.pre != PK_NORM_NONE) take(p.pre_gamma, hg);
     if (p.pre == PK_NORM_LAYER) take(p.pre_beta, hb);
-    if (!by_rows) {
+    if constexpr (!BY_ROWS) {
       float2 g[P];
 #pragma unroll
       for (int j = 0; j < P; ++j) g[j] = one;
@@ -372,32 +369,36 @@ __global__ void __launch_bounds__(RN_COLS, 1) residual_norm_rows_kernel(const Rn
       for (int j = 0; j < P; ++j) v[i][j] = make_float2(e[2 * j], e[2 * j + 1]);
       rstd[i] = 1.0f;
     }
-    uint4 xc[RN_R];
-#pragma unroll
-    for (int i = 0; i < RN_R; ++i) xc[i] = xr[i];
-    if (left > step) fetch(at + (int64_t)step * C, left - step);
+    const int64_t next = at + (int64_t)step * C;
+    if (left > step) fetch(p.f, next, left - step, fr);
     if (p.post != PK_NORM_NONE) normalize(p.post);
 #pragma unroll
     for (int i = 0; i < RN_R; ++i) {
       float e[VEC], y[VEC];
-      rn_unpack<T, VEC>(xc[i], e);
-      float2 w[P];
+      rn_unpack<T, VEC>(xr[i], e);
+      float2 w[P];  // the row's gate times the scale
 #pragma unroll
       for (int j = 0; j < P; ++j) w[j] = one;
-      if (by_rows && in && i < left) {
-        const float* gate = p.gate + (p.rows - left + i) / p.gate_rows * C + c;
+      if constexpr (BY_ROWS) {
+        if (in && i < left) {
+          const float* gate = p.gate + (size_t)((uint32_t)(p.rows - left + i) / gate_rows) * C + c;
 #pragma unroll
-        for (int j = 0; j < P; j += 2) {
-          const float4 g = __ldg(reinterpret_cast<const float4*>(gate + 2 * j));
-          w[j] = make_float2(g.x * p.scale, g.y * p.scale);
-          w[j + 1] = make_float2(g.z * p.scale, g.w * p.scale);
+          for (int j = 0; j < P; j += 2) {
+            const float4 g = __ldg(reinterpret_cast<const float4*>(gate + 2 * j));
+            w[j] = make_float2(g.x * p.scale, g.y * p.scale);
+            w[j + 1] = make_float2(g.z * p.scale, g.w * p.scale);
+          }
         }
       }
 #pragma unroll
       for (int j = 0; j < P; ++j) {
+        const float2 x = make_float2(e[2 * j], e[2 * j + 1]);
         float2 u = ffma2(v[i][j], make_float2(rstd[i], rstd[i]), zero);
-        u = ffma2(u, sg[j], sb[j]);
-        u = ffma2(u, w[j], make_float2(e[2 * j], e[2 * j + 1]));
+        if constexpr (BY_ROWS) {
+          u = ffma2(ffma2(u, sg[j], sb[j]), w[j], x);
+        } else {
+          u = ffma2(u, sg[j], ffma2(sb[j], one, x));
+        }
         v[i][j] = u;
         y[2 * j] = u.x;
         y[2 * j + 1] = u.y;
@@ -405,6 +406,7 @@ __global__ void __launch_bounds__(RN_COLS, 1) residual_norm_rows_kernel(const Rn
       if (in && i < left)
         *reinterpret_cast<uint4*>(static_cast<T*>(p.y) + at + (size_t)(uint32_t)(i * C)) = rn_pack<T, VEC>(y);
     }
+    if (left > step) fetch(p.x, next, left - step, xr);
     if (p.pre == PK_NORM_NONE) continue;
     normalize(p.pre);
 #pragma unroll
@@ -453,7 +455,8 @@ template <typename T>
 int launch_rows(const DeviceCtx& dev, const RnParams& p, cudaStream_t stream) {
   const int threads = (p.channels * (int)sizeof(T) / 16 + 31) / 32 * 32;
   const int64_t ctas = std::min<int64_t>((p.rows + RN_R - 1) / RN_R, (int64_t)dev.sm_count * (RN_COLS / threads));
-  return cuda_error(launch_kernel(residual_norm_rows_kernel<T>, dim3((unsigned)ctas), dim3((unsigned)threads), 0, stream, p),
+  auto kernel = p.gate && p.gate_rows > 0 ? residual_norm_rows_kernel<T, true> : residual_norm_rows_kernel<T, false>;
+  return cuda_error(launch_kernel(kernel, dim3((unsigned)ctas), dim3((unsigned)threads), 0, stream, p),
                     "residual_norm launch");
 }
 

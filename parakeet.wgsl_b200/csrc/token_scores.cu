@@ -46,6 +46,7 @@ constexpr int TS_MAXK = 32;              // one alternative per lane
 constexpr int TS_CLUSTER = 8;            // CTAs that share a row, at most
 constexpr int TS_HELD = 10;              // 16-byte vectors per lane of a held row, at most
 constexpr int TS_HELD_FEW = 4;           // and where there are few rows: more warps, shorter chains
+constexpr int TS_AGAIN = 2;              // lanes whose vectors are read again at a time
 constexpr int TS_UNR = 4;                // vectors per lane and tile of a streamed row
 constexpr int TS_POOL = 128;             // candidates per warp of a row
 constexpr uint32_t TS_MASKED = 0x007fffffu;  // ts_ordered(-inf)
@@ -472,12 +473,20 @@ __global__ void __launch_bounds__(TS_THREADS, sizeof(T) == 2 && NV > 0 ? (NV == 
       const uint32_t reach = __ballot_sync(0xffffffffu, m >= bound);
       const int own = first < vectors ? (vectors - first + step - 1) / step * TS_UNR : 0;
       auto again = [&](auto use) {
-        for (uint32_t lanes = reach; lanes; lanes &= lanes - 1) {
-          const int src = __ffs(lanes) - 1;
-          for (int i0 = 0; i0 < own; i0 += 32) {
-            const int i = i0 + lane;
-            const int v = i < own ? first + i / TS_UNR * step + 32 * (i % TS_UNR) + src : vectors;
-            use(TsTile<T, 1>::vector(base, skew, columns, v, vectors), v * VEC - skew);
+        for (int i0 = 0; i0 < own; i0 += 32) {
+          const int i = i0 + lane;
+          const int at = first + i / TS_UNR * step + 32 * (i % TS_UNR);
+          for (uint32_t lanes = reach; lanes;) {
+            uint4 raw[TS_AGAIN];
+            int v[TS_AGAIN];
+#pragma unroll
+            for (int n = 0; n < TS_AGAIN; ++n) {
+              v[n] = i < own && lanes ? at + __ffs(lanes) - 1 : vectors;
+              lanes &= lanes - 1;
+              raw[n] = TsTile<T, 1>::vector(base, skew, columns, v[n], vectors);
+            }
+#pragma unroll
+            for (int n = 0; n < TS_AGAIN; ++n) use(raw[n], v[n] * VEC - skew);
           }
         }
       };

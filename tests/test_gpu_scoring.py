@@ -531,7 +531,10 @@ def _joint(pk, device, counts, frames, max_tokens, inner, columns, profile, bias
     h = np.maximum(enc[i, np.minimum(at[i, u], frames - 1)].astype(np.float64) + pred[i, u], 0.0)
     w64 = w.astype(np.float64)
     v, mass = h @ w64 + (b if bias else 0.0), h @ np.abs(w64)
-    dv = (2.0 ** -11 + (inner / 16 + 8) * 2 * E) * mass if profile == "fp16" else (inner + 8) * E * mass
+    # FP16: hidden's rounding, and a step of 2^-23 per product instruction (16 inputs).  FP32: three tf32
+    # products a term, each of 8 inputs an instruction; the two low parts are cut at 2^-22 of their value and
+    # the product of the two is left out.
+    dv = (2.0 ** -11 + (inner / 16 + 8) * 2 * E if profile == "fp16" else 3 * 4 * E + (3 * inner / 8 + 8) * 2 * E) * mass
     dv = dv + 2 * E * np.abs(v)
     err = np.abs(_np(logits)[:n] - v) - (dv + HALF[profile] * (np.abs(v) + dv) + TINY[profile])
     assert np.all(err <= 0), float(err.max())
