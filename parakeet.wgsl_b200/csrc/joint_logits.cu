@@ -11,7 +11,7 @@
 //
 // Both precisions run on the tensor cores (tcgen05, f32 accumulators in TMEM).
 // A tile is 128 rows times up to 256 (FP32: 128) columns, whose width follows
-// from the number of row tiles, so that few rows still fill the SMs.  8 warps
+// from the number of row tiles, so that few rows still fill the SMs.  8 warps (FP32: 16)
 // gather, add, clamp and lay out 128 bytes of inputs a step in shared memory
 // (K-major, 128-byte swizzle), their loads two steps ahead; one warp issues the
 // MMAs, one the weights' loads, so that none of the three waits for another's
@@ -22,7 +22,8 @@
 // weight [inner, columns] arrives by TMA as it lies (the MN-major operand).
 // FP32: an f32 is the sum of two tf32 values up to 2^-22 of itself, so logits
 // are three tf32 products, hi hi + hi lo + lo hi (what is left out is 2^-22 of
-// a product).  The threads split the weights too, and lay them out K-major.
+// a product).  The threads split the weights too, from a TMA copy of them, and
+// lay them out K-major.
 // The MMA cuts its f32 sums, always towards zero, so one accumulator over all
 // 3 inner / 8 products drifts (4e-5 in logits of 12 at inner 640): the two
 // small products have an accumulator of their own, and the steps of the large
@@ -38,36 +39,43 @@
 namespace pk {
 namespace {
 
-constexpr int JL_ROWS = 256;       // threads that lay out rows and store logits
-constexpr int JL_THREADS = JL_ROWS + 64;  // and a warp each for the MMAs and the weights' loads
+constexpr int JL_ROWS = 512;       // threads that lay out rows and store logits, at most
 constexpr int JL_M = 128;          // rows per tile
 constexpr int JL_BAR = 192 * 1024;  // after the stages: the barriers
-constexpr int JL_MISC = JL_BAR + 128;
+constexpr int JL_MISC = JL_BAR + 256;
 constexpr int JL_SMEM = JL_MISC + 64 + 1024;  // + alignment slack
 static_assert(JL_SMEM <= 232448, "shared memory budget");
 // A stage: FP16 the rows (16 KB) and the weights (32 KB), FP32 hi and lo of both (16 KB each).
 template <typename T>
-constexpr int jl_stages() { return sizeof(T) == 2 ? 4 : 3; }
+constexpr int jl_stages() { return sizeof(T) == 2 ? 4 : 2; }
 template <typename T>
-constexpr int jl_stage() { return JL_BAR / jl_stages<T>(); }
+constexpr int jl_stage() { return sizeof(T) == 2 ? 48 * 1024 : 64 * 1024; }
 template <typename T>
 constexpr int jl_b() { return sizeof(T) == 2 ? 16 * 1024 : 32 * 1024; }  // the weights of a stage
-static_assert(jl_stage<__half>() % 1024 == 0 && jl_stage<float>() % 1024 == 0, "swizzled operands start on 1024 bytes");
+// FP32: the weights as they lie, [32 inputs][128 columns], behind the stages.
+constexpr int JL_RAW = 128 * 1024, JL_RAW_STAGES = 4, JL_RAW_STAGE = 16 * 1024;
+static_assert(JL_RAW == jl_stages<float>() * jl_stage<float>() && JL_RAW + JL_RAW_STAGES * JL_RAW_STAGE <= JL_BAR &&
+              jl_stages<__half>() * jl_stage<__half>() <= JL_BAR, "stages fit");
 template <typename T>
 constexpr int jl_k() { return 128 / (int)sizeof(T); }  // inputs per step: 128 bytes
 constexpr int JL_TMEM = 512;       // TMEM columns: FP32's accumulators (FP16: 256 are enough)
 template <typename T>
 constexpr int jl_ahead() { return 2; }  // steps whose inputs are on their way to registers
+// Row threads: FP32 has the weights to lay out too.  A warp each for the MMAs
+// and the weights' loads comes after them.
+template <typename T>
+constexpr int jl_rows() { return sizeof(T) == 2 ? 256 : 512; }
 template <typename T>
 constexpr int jl_n() { return sizeof(T) == 2 ? 256 : 128; }  // columns per tile, at most
 
 struct JlParams {
-  CUtensorMap tmap_w;  // weight [inner][columns] f16, box {64, 64}, 128-byte swizzle (reads past the edge are 0)
+  // weight [inner][columns]; reads past the edge are 0.  FP16: box {64, 64},
+  // 128-byte swizzle; FP32: box {128, 32}, as it lies.
+  CUtensorMap tmap_w;
   const void* encoder;
   const float* predictor;
   const uint32_t* joint_frames;
   const uint32_t* counts;
-  const void* weight;
   const float* bias;
   void* logits;
   uint32_t* row_map;
@@ -84,10 +92,12 @@ struct JlRows {
   int warp_sum[JL_ROWS / 32];
 };
 
-__device__ __forceinline__ void jl_rows_sync() { asm volatile("bar.sync 1, %0;" ::"n"(JL_ROWS) : "memory"); }
+template <int ROWS>
+__device__ __forceinline__ void jl_rows_sync() { asm volatile("bar.sync 1, %0;" ::"n"(ROWS) : "memory"); }
 
 // The row threads: windows w0 + tid, whose rows come after `base` others.  Fills
 // rows.start and returns the number of rows up to the last of these windows.
+template <int ROWS>
 __device__ __forceinline__ int jl_scan(const JlParams& p, JlRows& rows, int w0, int base) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n = w0 + tid < p.batch ? (int)min(p.counts[w0 + tid], (uint32_t)p.max_tokens) : 0;
@@ -98,44 +108,45 @@ __device__ __forceinline__ int jl_scan(const JlParams& p, JlRows& rows, int w0, 
     if (lane >= o) incl += v;
   }
   if (lane == 31) rows.warp_sum[warp] = incl;
-  jl_rows_sync();
-  const int sum = lane < JL_ROWS / 32 ? rows.warp_sum[lane] : 0;
+  jl_rows_sync<ROWS>();
+  const int sum = lane < ROWS / 32 ? rows.warp_sum[lane] : 0;
   rows.start[tid] = base + __reduce_add_sync(0xffffffffu, lane < warp ? sum : 0) + incl - n;
-  jl_rows_sync();
+  jl_rows_sync<ROWS>();
   return base + __reduce_add_sync(0xffffffffu, sum);
 }
 
 // The row threads: places and frames of rows [r0, r0 + JL_M) and the bias from
-// column n0 on.  `all`: rows of the first JL_ROWS windows, whose starts
+// column n0 on.  `all`: rows of the first ROWS windows, whose starts
 // are in rows.start where they are all the windows.
+template <int ROWS>
 __device__ __forceinline__ void jl_fill(const JlParams& p, JlRows& rows, int r0, int n0, int all) {
   const int tid = threadIdx.x;
-  jl_rows_sync();  // the previous tile's are read
+  jl_rows_sync<ROWS>();  // the previous tile's are read
   rows.bias[tid] = p.bias && n0 + tid < p.columns ? __ldg(p.bias + n0 + tid) : 0.0f;
   int place = -1;
   int base = 0;
-  if (p.batch > JL_ROWS) all = jl_scan(p, rows, 0, 0);
-  for (int w0 = 0;; w0 += JL_ROWS) {
+  if (p.batch > ROWS) all = jl_scan<ROWS>(p, rows, 0, 0);
+  for (int w0 = 0;; w0 += ROWS) {
     const int r = r0 + tid;
     if (tid < JL_M && r >= base && r < all) {
       // The last window that starts at or before r (windows without rows start where the next does).
       int w = 0;
 #pragma unroll
-      for (int step = JL_ROWS / 2; step > 0; step >>= 1)
+      for (int step = ROWS / 2; step > 0; step >>= 1)
         if (rows.start[w + step] <= r) w += step;
       place = (w0 + w) * p.max_tokens + r - rows.start[w];
     }
-    if (w0 + JL_ROWS >= p.batch) break;
-    jl_rows_sync();
+    if (w0 + ROWS >= p.batch) break;
+    jl_rows_sync<ROWS>();
     base = all;
-    all = jl_scan(p, rows, w0 + JL_ROWS, base);
+    all = jl_scan<ROWS>(p, rows, w0 + ROWS, base);
   }
   if (tid < JL_M) {
     rows.place[tid] = place;
     if (place >= 0)
       rows.frame[tid] = place / p.max_tokens * p.frames + (int)min(p.joint_frames[place], (uint32_t)(p.frames - 1));
   }
-  jl_rows_sync();
+  jl_rows_sync<ROWS>();
 }
 
 __device__ __forceinline__ float jl_relu(float v) { return v < 0.0f ? 0.0f : v; }  // keeps NaN
@@ -144,72 +155,75 @@ __device__ __forceinline__ uint32_t jl_hidden2(uint32_t e, float p0, float p1) {
   const __half2 h = __floats2half2_rn(jl_relu(f.x + p0), jl_relu(f.y + p1));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// The leading 11 bits of v (a tf32 value), and the rest.  An infinite v has no rest.
+// The leading 11 bits of v (a tf32 value), and the rest (NaN for an infinite v).
 __device__ __forceinline__ void jl_split(float v, uint32_t& hi, uint32_t& lo) {
   hi = __float_as_uint(v) & 0xffffe000u;
-  if (v != v) hi = 0x7fc00000u;
-  const float d = v - __uint_as_float(hi);
-  lo = d == d ? __float_as_uint(d) : 0u;
+  lo = __float_as_uint(v - __uint_as_float(hi));
 }
 // 16-byte chunk `c` of row `r` in a K-major block of 128-byte rows, swizzled.
 __device__ __forceinline__ uint32_t jl_at(int r, int c) {
   return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
 }
 
-// What a thread gathers for one step: chunk tid % 8 of rows tid / 8 + 32 i, and
-// (FP32) inputs 4 (tid / 128) + 8 i .. + 3 of column tid % 128 of the weights.
-constexpr int JL_TASKS = JL_M * 8 / JL_ROWS;
+// What a thread gathers for one step: chunk tid % 8 of every 32nd (FP32: 64th) row.
+template <typename T>
+constexpr int jl_tasks() { return JL_M * 8 / jl_rows<T>(); }
 template <typename T>
 struct JlSlot;
 template <>
 struct JlSlot<__half> {
-  uint4 e[JL_TASKS];
-  float4 p[JL_TASKS][2];
+  uint4 e[jl_tasks<__half>()];
+  float4 p[jl_tasks<__half>()][2];
 };
 template <>
 struct JlSlot<float> {
-  float4 e[JL_TASKS], p[JL_TASKS];
-  float w[JL_TASKS][4];
+  float4 e[jl_tasks<float>()], p[jl_tasks<float>()];
 };
 
 template <typename T>
-__global__ void __launch_bounds__(JL_THREADS, 1) joint_logits_kernel(const __grid_constant__ JlParams p) {
+__global__ void __launch_bounds__(jl_rows<T>() + 64, 1) joint_logits_kernel(const __grid_constant__ JlParams p) {
   pdl_entry();
   extern __shared__ uint8_t jl_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(jl_raw) + 1023) & ~uintptr_t(1023));
   __shared__ JlRows rows;
   constexpr bool F16 = sizeof(T) == 2;
+  constexpr int ROWS = jl_rows<T>(), TASKS = jl_tasks<T>();
   constexpr int K = jl_k<T>(), N = jl_n<T>(), EPC = 16 / sizeof(T);  // elements per chunk
   constexpr int STAGES = jl_stages<T>(), STAGE = jl_stage<T>(), B = jl_b<T>();
+  constexpr int RAW = F16 ? STAGES : JL_RAW_STAGES;  // the weights' stages (FP16: the MMAs')
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + JL_BAR);  // the stage's rows are laid out
-  uint64_t* weights = full + STAGES;                          // FP16: the stage's weights have landed
-  uint64_t* empty = weights + STAGES;                         // the stage's MMAs have read it
+  uint64_t* weights = full + STAGES;                          // the weights' stage has landed
+  uint64_t* unpacked = weights + RAW;                         // FP32: the row threads have read it
+  uint64_t* empty = unpacked + RAW;                           // the stage's MMAs have read it
   uint64_t* done = empty + STAGES;                            // the tile's MMAs are complete
   uint64_t* taken = done + 1;                                 // the tile's accumulators are read
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + JL_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + JL_MISC + 4);
   int* totals = reinterpret_cast<int*>(sm + JL_MISC + 8);
-  if (tid == JL_ROWS) {
+  if (tid == ROWS) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&full[i], JL_ROWS / 32);
-      mbar_init(&weights[i], 1);
+      mbar_init(&full[i], ROWS / 32);
       mbar_init(&empty[i], 1);
     }
+    for (int i = 0; i < RAW; ++i) {
+      mbar_init(&weights[i], 1);
+      mbar_init(&unpacked[i], ROWS / 32);
+    }
     mbar_init(done, 1);
-    mbar_init(taken, JL_ROWS / 32);
+    mbar_init(taken, ROWS / 32);
     *abort_flag = 0;
     fence_mbar_init();
-    if constexpr (F16) tma_prefetch_desc(&p.tmap_w);
+    tma_prefetch_desc(&p.tmap_w);
   }
-  if (warp == JL_ROWS / 32 + 1) {
+  if (warp == ROWS / 32 + 1) {
     tmem_alloc(tmem_slot, F16 ? N : JL_TMEM);
     tmem_relinquish();
   }
-  if (tid < JL_ROWS) {
-    const int all = jl_scan(p, rows, 0, 0);
+  if (tid < ROWS) {
+    const int all = jl_scan<ROWS>(p, rows, 0, 0);
     int total = all;
-    for (int w0 = JL_ROWS; w0 < p.batch; w0 += JL_ROWS) total = jl_scan(p, rows, w0, total);
+    for (int w0 = ROWS; w0 < p.batch; w0 += ROWS) total = jl_scan<ROWS>(p, rows, w0, total);
     if (tid == 0) {
       totals[0] = total;
       totals[1] = all;
@@ -237,7 +251,7 @@ __global__ void __launch_bounds__(JL_THREADS, 1) joint_logits_kernel(const __gri
   // used % STAGES.  A wait that expires raises the abort flag and ends the
   // roles' loops; they meet again behind them.
   uint32_t used = 0;
-  if (warp == JL_ROWS / 32) {
+  if (warp == ROWS / 32) {
     // ------------------------------------------------------------ MMAs
     if (lane == 0) {
       const uint32_t idesc = (F16 ? umma_idesc_f16(JL_M, 0, 0, /*weight, MN-major*/ 1) : umma_idesc_tf32(JL_M, 0)) |
@@ -278,25 +292,26 @@ __global__ void __launch_bounds__(JL_THREADS, 1) joint_logits_kernel(const __gri
       // Unwind: the MMAs issued are complete before the roles meet.
       if (!good && used > 0) mbar_wait_drain(&empty[(used - 1) % STAGES], (used - 1) / STAGES & 1, p.status);
     }
-  } else if (warp == JL_ROWS / 32 + 1) {
-    // ------------------------------------------------------------ weights (FP16)
-    if (F16 && lane == 0) {
-      const int boxes = (bn + 63) / 64;
+  } else if (warp == ROWS / 32 + 1) {
+    // ------------------------------------------------------------ weights
+    if (lane == 0) {
+      const int boxes = F16 ? (bn + 63) / 64 : 1;
+      uint64_t* read = F16 ? empty : unpacked;
       bool good = true;
       for (int tile = blockIdx.x; tile < tiles && good; tile += gridDim.x) {
         const int n0 = tile % ntiles * bn;
         for (int kb = 0; kb < steps; ++kb, ++used) {
-          const uint32_t st = used % STAGES, use = used / STAGES;
-          if (use > 0) good = mbar_wait(&empty[st], (use - 1) & 1, abort_flag, p.status, PK_STATUS_TIMEOUT_MMA);
+          const uint32_t st = used % RAW, use = used / RAW;
+          if (use > 0) good = mbar_wait(&read[st], (use - 1) & 1, abort_flag, p.status, PK_STATUS_TIMEOUT_MMA);
           if (!good) break;
-          mbar_arrive_expect_tx(&weights[st], (uint32_t)boxes * K * 128);
-          for (int b = 0; b < boxes; ++b)
-            tma_load_2d(sm + st * STAGE + B + b * K * 128, &p.tmap_w, &weights[st], n0 + 64 * b, kb * K);
+          mbar_arrive_expect_tx(&weights[st], (uint32_t)(F16 ? boxes * K * 128 : JL_RAW_STAGE));
+          uint8_t* dst = F16 ? sm + st * STAGE + B : sm + JL_RAW + st * JL_RAW_STAGE;
+          for (int b = 0; b < boxes; ++b) tma_load_2d(dst + b * K * 128, &p.tmap_w, &weights[st], n0 + 64 * b, kb * K);
         }
       }
       // Unwind: the loads issued have landed before the roles meet.
-      for (uint32_t s = 0; s < STAGES; ++s)
-        if (used > s) mbar_wait_drain(&weights[s], (used - s - 1) / STAGES & 1, p.status);
+      for (uint32_t s = 0; s < RAW; ++s)
+        if (used > s) mbar_wait_drain(&weights[s], (used - s - 1) / RAW & 1, p.status);
     }
   } else {
     // ------------------------------------------------------------ rows and logits
@@ -307,26 +322,23 @@ __global__ void __launch_bounds__(JL_THREADS, 1) joint_logits_kernel(const __gri
     bool good = true;  // of this warp
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++turn) {
       const int r0 = tile / ntiles * JL_M, n0 = tile % ntiles * bn;
-      jl_fill(p, rows, r0, n0, all);
+      jl_fill<ROWS>(p, rows, r0, n0, all);
       if (n0 == 0 && tid < JL_M && rows.place[tid] >= 0) p.row_map[r0 + tid] = (uint32_t)rows.place[tid];
-      const T* es[JL_TASKS];
-      const float* ps[JL_TASKS];
-      bool live[JL_TASKS];
+      const T* es[TASKS];
+      const float* ps[TASKS];
+      bool live[TASKS];
 #pragma unroll
-      for (int i = 0; i < JL_TASKS; ++i) {
-        const int place = rows.place[rbase + 32 * i];
+      for (int i = 0; i < TASKS; ++i) {
+        const int place = rows.place[rbase + ROWS / 8 * i];
         live[i] = place >= 0;
-        es[i] = enc + (size_t)(live[i] ? rows.frame[rbase + 32 * i] : 0) * p.inner + chunk * EPC;
+        es[i] = enc + (size_t)(live[i] ? rows.frame[rbase + ROWS / 8 * i] : 0) * p.inner + chunk * EPC;
         ps[i] = p.predictor + (size_t)(live[i] ? place : 0) * p.inner + chunk * EPC;
       }
       const int wn = tid & 127, wk = tid >> 7;  // FP32: this thread's column and inputs of a step's weights
-      const float* ws = static_cast<const float*>(p.weight) + (size_t)(4 * wk) * p.columns + n0 + wn;
-      const bool wlive = wn < bn && n0 + wn < p.columns;
       auto fetch = [&](JlSlot<T>& s, int kb) {
         const int k = kb * K;
-        const float* wp = ws + (size_t)k * p.columns;
 #pragma unroll
-        for (int i = 0; i < JL_TASKS; ++i) {
+        for (int i = 0; i < TASKS; ++i) {
           const bool in = live[i] && k + chunk * EPC < p.inner;
           if constexpr (F16) {
             s.e[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -342,10 +354,6 @@ __global__ void __launch_bounds__(JL_THREADS, 1) joint_logits_kernel(const __gri
               s.e[i] = *reinterpret_cast<const float4*>(es[i] + k);
               s.p[i] = *reinterpret_cast<const float4*>(ps[i] + k);
             }
-            // inner is a multiple of 32, a step's inputs are all inside
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              s.w[i][j] = wlive ? __ldg(wp + (uint32_t)(8 * i + j) * (uint32_t)p.columns) : 0.0f;
           }
         }
       };
@@ -362,12 +370,13 @@ __global__ void __launch_bounds__(JL_THREADS, 1) joint_logits_kernel(const __gri
             const uint32_t st = used % STAGES, use = used / STAGES;
             uint8_t* stage = sm + st * STAGE;
             if (use > 0 && good) good = mbar_wait(&empty[st], (use - 1) & 1, abort_flag, p.status, PK_STATUS_TIMEOUT_MMA);
+            if (!F16 && good) good = mbar_wait(&weights[used % RAW], used / RAW & 1, abort_flag, p.status, PK_STATUS_TIMEOUT_TMA);
             good = __all_sync(0xffffffffu, good);
             JlSlot<T>& s = slot[d];
             if (good) {
 #pragma unroll
-              for (int i = 0; i < JL_TASKS; ++i) {
-                const uint32_t at = jl_at(rbase + 32 * i, chunk);
+              for (int i = 0; i < TASKS; ++i) {
+                const uint32_t at = jl_at(rbase + ROWS / 8 * i, chunk);
                 if constexpr (F16) {
                   uint4 o;
                   o.x = jl_hidden2(s.e[i].x, s.p[i][0].x, s.p[i][0].y);
@@ -383,16 +392,28 @@ __global__ void __launch_bounds__(JL_THREADS, 1) joint_logits_kernel(const __gri
                   jl_split(jl_relu(s.e[i].w + s.p[i].w), hi.w, lo.w);
                   *reinterpret_cast<uint4*>(stage + at) = hi;
                   *reinterpret_cast<uint4*>(stage + JL_M * 128 + at) = lo;
-                  if (wn < bn) {
-                    const uint32_t wat = jl_at(wn, wk + 2 * i);
-                    jl_split(s.w[i][0], hi.x, lo.x);
-                    jl_split(s.w[i][1], hi.y, lo.y);
-                    jl_split(s.w[i][2], hi.z, lo.z);
-                    jl_split(s.w[i][3], hi.w, lo.w);
+                }
+              }
+              if constexpr (!F16) {
+                const float* raw = reinterpret_cast<const float*>(sm + JL_RAW + used % RAW * JL_RAW_STAGE) + wn;
+                if (wn < bn) {
+#pragma unroll
+                  for (int i = 0; i < K / 16; ++i) {  // 16 inputs at a time over the row threads
+                    float w[4];
+                    uint4 hi, lo;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[j] = raw[(4 * wk + 16 * i + j) * N];
+                    jl_split(w[0], hi.x, lo.x);
+                    jl_split(w[1], hi.y, lo.y);
+                    jl_split(w[2], hi.z, lo.z);
+                    jl_split(w[3], hi.w, lo.w);
+                    const uint32_t wat = jl_at(wn, wk + 4 * i);
                     *reinterpret_cast<uint4*>(stage + B + wat) = hi;
                     *reinterpret_cast<uint4*>(stage + B + N * 128 + wat) = lo;
                   }
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&unpacked[used % RAW]);
               }
               fence_proxy_async_smem();
               __syncwarp();
@@ -407,28 +428,28 @@ __global__ void __launch_bounds__(JL_THREADS, 1) joint_logits_kernel(const __gri
       good = __all_sync(0xffffffffu, good);
       if (good) {
         tc_fence_after();
-        // Warp w reads TMEM lanes 32 (w % 4) .. + 31, columns 32 (w / 4) + 64 i .. + 31.
+        // Warp w reads TMEM lanes 32 (w % 4) .. + 31, columns 16 (w / 4) + ROWS / 8 i .. + 15.
         const int r = (warp & 3) * 32 + lane;
         const bool mine = rows.place[r] >= 0;
         T* out = static_cast<T*>(p.logits) + (size_t)(r0 + r) * p.columns;
-        for (int c = (warp >> 2) * 32; c < bn; c += 64) {
-          uint32_t v[32];
+        for (int c = (warp >> 2) * 16; c < bn; c += ROWS / 8) {
+          uint32_t v[16];
           const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c;
-          tc_ld_32x32b_x32(at, v);
+          tc_ld_32x32b_x16(at, v);
           tc_wait_ld();
           if constexpr (!F16) {
             for (int a = 1; a <= turns; ++a) {
-              uint32_t u[32];
-              tc_ld_32x32b_x32(at + (uint32_t)(a * pitch), u);
+              uint32_t u[16];
+              tc_ld_32x32b_x16(at + (uint32_t)(a * pitch), u);
               tc_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(u[j]));
+              for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(u[j]));
             }
           }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 2; ++q) {
             const int n = n0 + c + 8 * q;
-            if (mine && c + 8 * q < bn && n < p.columns) {  // columns are a multiple of 8
+            if (mine && n < p.columns) {  // columns are a multiple of 8, a tile's of 16
               float b[8];
               *reinterpret_cast<float4*>(b) = *reinterpret_cast<const float4*>(rows.bias + c + 8 * q);
               *reinterpret_cast<float4*>(b + 4) = *reinterpret_cast<const float4*>(rows.bias + c + 8 * q + 4);
@@ -454,7 +475,7 @@ __global__ void __launch_bounds__(JL_THREADS, 1) joint_logits_kernel(const __gri
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == JL_ROWS / 32 + 1) {
+  if (warp == ROWS / 32 + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, F16 ? N : JL_TMEM);
   }
@@ -466,7 +487,7 @@ int launch_typed(const DeviceCtx& dev, const JlParams& p, cudaStream_t stream) {
   if (st != PK_OK) return st;
   const int64_t tiles = ((int64_t)p.batch * p.max_tokens + JL_M - 1) / JL_M * ((p.columns + 63) / 64);
   return cuda_error(launch_kernel(joint_logits_kernel<T>, dim3((unsigned)std::min<int64_t>(tiles, dev.sm_count)),
-                                  dim3(JL_THREADS), JL_SMEM, stream, p),
+                                  dim3(jl_rows<T>() + 64), JL_SMEM, stream, p),
                     "joint_logits launch");
 }
 
@@ -478,7 +499,6 @@ int launch_joint_logits(const DeviceCtx& dev, const pk_joint_logits_desc& d, cud
   p.predictor = d.predictor;
   p.joint_frames = d.joint_frames;
   p.counts = d.counts;
-  p.weight = d.weight;
   p.bias = d.bias;
   p.logits = d.logits;
   p.row_map = d.row_map;
@@ -489,16 +509,19 @@ int launch_joint_logits(const DeviceCtx& dev, const pk_joint_logits_desc& d, cud
   p.max_tokens = d.max_tokens;
   p.inner = (int)d.inner;
   p.columns = (int)d.columns;
-  if (d.precision == PK_FP32) return launch_typed<float>(dev, p, stream);
+  const bool f16 = d.precision == PK_FP16;
   auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(dev.encode_tiled);
   const cuuint64_t dims[2] = {(cuuint64_t)p.columns, (cuuint64_t)p.inner};
-  const cuuint64_t strides[1] = {(cuuint64_t)p.columns * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)jl_k<__half>()}, unit[2] = {1, 1};
+  const cuuint64_t strides[1] = {(cuuint64_t)p.columns * (f16 ? 2 : 4)};
+  const cuuint32_t box16[2] = {64, (cuuint32_t)jl_k<__half>()}, box32[2] = {(cuuint32_t)jl_n<float>(), (cuuint32_t)jl_k<float>()};
+  const cuuint32_t unit[2] = {1, 1};
   if (!encode ||
-      encode(&p.tmap_w, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(d.weight), dims, strides, box, unit,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      encode(&p.tmap_w, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2,
+             const_cast<void*>(d.weight), dims, strides, f16 ? box16 : box32, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             f16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return set_error(PK_E_CUDA, "cuTensorMapEncodeTiled failed (joint weight)");
+  if (!f16) return launch_typed<float>(dev, p, stream);
   return launch_typed<__half>(dev, p, stream);
 }
 
