@@ -225,6 +225,19 @@ typedef struct pk_tdt_desc {
 } pk_tdt_desc;
 int pk_tdt_decode(pk_device* device, const pk_tdt_desc* desc, pk_stream stream);
 
+/* pk_tdt_decode that also leaves what the joint saw at every emission u of
+ * window w: predictor[w, u] is the projected prediction net after the u
+ * tokens before it, joint_frames[w, u] the encoder frame of the joint (the
+ * flush looks at other frames than it emits at).  The tokens are those of
+ * pk_tdt_decode.  What lies behind a window's emissions is not specified.  No
+ * counterpart in the reference; pk_joint_logits and pk_token_scores turn it
+ * into the emissions' probabilities. */
+typedef struct pk_tdt_trace {
+  float* predictor;          /* device f32 [batch, max_tokens, 640] */
+  uint32_t* joint_frames;    /* device u32 [batch, max_tokens] */
+} pk_tdt_trace;
+int pk_tdt_decode_traced(pk_device* device, const pk_tdt_desc* desc, const pk_tdt_trace* trace, pk_stream stream);
+
 /* ------------------------------------------------------------- scoring
  * A decoder's last steps, from a block's output to a scored answer.  No
  * counterparts in the reference, which returns token ids alone.  No entry

@@ -36,6 +36,7 @@ EXPORTED = (
     "pk_debug_wait_probe", "pk_stitch_create", "pk_stitch_destroy", "pk_stitch_append", "pk_stitch_append_tdt",
     "pk_stitch_extend", "pk_stitch_counts", "pk_stitch_read", "pk_stitch_read_run",
     "pk_debug_set_reference_arithmetic", "pk_token_scores", "pk_residual_norm", "pk_int4_gemv", "pk_joint_logits",
+    "pk_tdt_decode_traced",
 )
 STITCH_COLLECT_TRACE, STITCH_RECORD_RUN = 1, 2
 
@@ -119,6 +120,10 @@ class JointLogitsDesc(ctypes.Structure):
                                         "logits", "row_map", "row_count")]
 
 
+class TdtTrace(ctypes.Structure):
+    _fields_ = [("predictor", ctypes.c_void_p), ("joint_frames", ctypes.c_void_p)]
+
+
 class TensorDesc(ctypes.Structure):
     _fields_ = [
         ("name", ctypes.c_char_p), ("dtype", ctypes.c_int), ("ndim", ctypes.c_int),
@@ -157,6 +162,7 @@ def load() -> ctypes.CDLL:
             "pk_subsampling_depthwise": [vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp, vp],
             "pk_subsampling_time_mask": [vp, i32, i32, i32, i32, i32, vp, vp, i32, vp],
             "pk_tdt_decode": [vp, ctypes.POINTER(TdtDesc), vp],
+            "pk_tdt_decode_traced": [vp, ctypes.POINTER(TdtDesc), ctypes.POINTER(TdtTrace), vp],
             "pk_logmel": [vp, i32, i32, vp, vp, vp, vp],
             "pk_token_scores": [vp, ctypes.POINTER(TokenScoresDesc), vp],
             "pk_residual_norm": [vp, ctypes.POINTER(ResidualNormDesc), vp],

@@ -291,7 +291,7 @@ int pk_logmel(pk_device* device, int batch, int sample_count, const float* sampl
   return launch_logmel(batch, sample_count, samples, valid_samples, features, as_stream(stream));
 }
 
-int pk_tdt_decode(pk_device* device, const pk_tdt_desc* d, pk_stream stream) {
+static int tdt_decode(pk_device* device, const pk_tdt_desc* d, const pk_tdt_trace& trace, pk_stream stream) {
   if (!device || !d) return set_error(PK_E_INVALID, "null argument");
   if (d->precision != PK_FP16 && d->precision != PK_FP32) return set_error(PK_E_INVALID, "unknown precision");
   if (d->batch <= 0 || d->batch > 16383) return set_error(PK_E_SHAPE, "Invalid TDT decoder batchSize");
@@ -311,10 +311,19 @@ int pk_tdt_decode(pk_device* device, const pk_tdt_desc* d, pk_stream stream) {
       return set_error(PK_E_LAYOUT, "TDT decoder weights and encoder input must be 16-byte aligned");
   cudaSetDevice(device->ctx.ordinal);
   if (g_decoder_route != 1) {
-    const int st = launch_tdt_resident(device->ctx, *d, as_stream(stream));
+    const int st = launch_tdt_resident(device->ctx, *d, trace, as_stream(stream));
     if (st != PK_E_SHAPE || g_decoder_route == 2) return st;
   }
-  return launch_tdt_decode(device->ctx, *d, as_stream(stream));
+  return launch_tdt_decode(device->ctx, *d, trace, as_stream(stream));
+}
+
+int pk_tdt_decode(pk_device* device, const pk_tdt_desc* d, pk_stream stream) {
+  return tdt_decode(device, d, pk_tdt_trace{nullptr, nullptr}, stream);
+}
+
+int pk_tdt_decode_traced(pk_device* device, const pk_tdt_desc* d, const pk_tdt_trace* trace, pk_stream stream) {
+  if (!trace || !trace->predictor || !trace->joint_frames) return set_error(PK_E_INVALID, "TDT trace pointer is null");
+  return tdt_decode(device, d, *trace, stream);
 }
 
 int pk_debug_set_decoder_route(int route) {

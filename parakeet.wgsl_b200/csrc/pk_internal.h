@@ -123,10 +123,11 @@ int launch_residual_norm(const DeviceCtx& dev, const pk_residual_norm_desc& d, c
 int launch_int4_gemv(const DeviceCtx& dev, const pk_int4_gemv_desc& d, cudaStream_t stream);
 int launch_joint_logits(const DeviceCtx& dev, const pk_joint_logits_desc& d, cudaStream_t stream);
 
-int launch_tdt_decode(const DeviceCtx& dev, const pk_tdt_desc& d, cudaStream_t stream);
+// trace: the joint's inputs at every emission (both pointers null: none).
+int launch_tdt_decode(const DeviceCtx& dev, const pk_tdt_desc& d, const pk_tdt_trace& trace, cudaStream_t stream);
 // Resident FP16 decoder (all windows in lockstep on 128 co-resident CTAs);
 // returns PK_E_SHAPE when it does not apply (then the cluster kernel runs).
-int launch_tdt_resident(const DeviceCtx& dev, const pk_tdt_desc& d, cudaStream_t stream);
+int launch_tdt_resident(const DeviceCtx& dev, const pk_tdt_desc& d, const pk_tdt_trace& trace, cudaStream_t stream);
 // Test knob: 0 = automatic, 1 = cluster kernel only, 2 = resident kernel only.
 extern int g_decoder_route;
 int launch_logmel(int batch, int sample_count, const float* samples, const uint32_t* valid_samples, float* features,

@@ -113,6 +113,7 @@ struct TdtPlan {
   int token;
   int joint;    // another joint follows
   int joint_t;  // its encoder frame
+  int count;    // tokens emitted so far
 };
 
 template <typename T>
@@ -166,6 +167,8 @@ struct TdtParams {
   uint32_t* token_frames;
   uint32_t* token_durations;
   uint32_t* metadata;
+  float* trace_predictor;  // [batch, max_tokens, 640], or null: the joint's inputs at every emission
+  uint32_t* trace_frames;  // [batch, max_tokens]
   unsigned int* status;
   int batch;
   int frames;
@@ -477,6 +480,10 @@ __device__ void consume_update(Ctx<T>& c, const TdtPlan& pl) {
       consume_end(c);
     }
     if (act) {
+      if (c.p.trace_predictor && pl.count < c.p.max_tokens) {
+        const size_t at = ((size_t)(blockIdx.x / TCL) * c.p.max_tokens + pl.count) * TH + o;
+        *reinterpret_cast<float2*>(c.p.trace_predictor + at) = acc;
+      }
       const uint32_t a = smem_addr(c.s.proj + o);
 #pragma unroll
       for (int r = 0; r < TCL; ++r) {
@@ -659,8 +666,8 @@ __global__ void __launch_bounds__(TTHREADS, 1) tdt_decoder_kernel(const __grid_c
   if (tid == 0) {
     enc_len = min(len_c, p.ends[window]);
     t = min(p.starts[window], enc_len);
-    TdtPlan pl{0, 0, 0, 0, 0};
-    if (t < enc_len) pl = TdtPlan{1, 1, 0, 1, (int)t};
+    TdtPlan pl{0, 0, 0, 0, 0, 0};
+    if (t < enc_len) pl = TdtPlan{1, 1, 0, 1, (int)t, 0};
     s.plan = pl;
   }
   block_sync();
@@ -694,13 +701,14 @@ __global__ void __launch_bounds__(TTHREADS, 1) tdt_decoder_kernel(const __grid_c
               p.tokens[o] = tok;
               p.token_frames[o] = frame;
               p.token_durations[o] = dur;
+              if (p.trace_frames) p.trace_frames[o] = (uint32_t)pl.joint_t;
             }
             ++count;
           } else {
             flags |= 1u;
           }
         };
-        TdtPlan next{nonblank ? 1 : 0, 0, (int)tok, 0, 0};
+        TdtPlan next{nonblank ? 1 : 0, 0, (int)tok, 0, 0, 0};
         if (mode == 0) {
           if (nonblank) emit(t);
           sym += 1;
@@ -743,6 +751,7 @@ __global__ void __launch_bounds__(TTHREADS, 1) tdt_decoder_kernel(const __grid_c
           }
         }
         if (!next.joint) next.lstm = 0;  // the shader's last update feeds nothing
+        next.count = (int)count;
         s.plan = next;
         s.first_exc = TH;
       }
@@ -786,7 +795,7 @@ bool encode_map(const DeviceCtx& dev, CUtensorMap* map, CUtensorMapDataType type
 }
 
 template <typename T>
-int launch_tdt_typed(const DeviceCtx& dev, const pk_tdt_desc& d, cudaStream_t stream) {
+int launch_tdt_typed(const DeviceCtx& dev, const pk_tdt_desc& d, const pk_tdt_trace& trace, cudaStream_t stream) {
   const CUtensorMapDataType type = sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   const cuuint64_t es = sizeof(T);
   TdtParams p;
@@ -828,6 +837,8 @@ int launch_tdt_typed(const DeviceCtx& dev, const pk_tdt_desc& d, cudaStream_t st
   p.token_frames = d.token_frames;
   p.token_durations = d.token_durations;
   p.metadata = d.metadata;
+  p.trace_predictor = trace.predictor;
+  p.trace_frames = trace.joint_frames;
   p.status = dev.status;
   p.batch = d.batch;
   p.frames = d.frames;
@@ -854,8 +865,9 @@ int launch_tdt_typed(const DeviceCtx& dev, const pk_tdt_desc& d, cudaStream_t st
 
 }  // namespace
 
-int launch_tdt_decode(const DeviceCtx& dev, const pk_tdt_desc& d, cudaStream_t stream) {
-  return d.precision == PK_FP16 ? launch_tdt_typed<__half>(dev, d, stream) : launch_tdt_typed<float>(dev, d, stream);
+int launch_tdt_decode(const DeviceCtx& dev, const pk_tdt_desc& d, const pk_tdt_trace& trace, cudaStream_t stream) {
+  return d.precision == PK_FP16 ? launch_tdt_typed<__half>(dev, d, trace, stream)
+                                : launch_tdt_typed<float>(dev, d, trace, stream);
 }
 
 }  // namespace pk

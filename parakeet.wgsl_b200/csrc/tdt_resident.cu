@@ -186,6 +186,8 @@ struct RParams {
   uint32_t* token_frames;
   uint32_t* token_durations;
   uint32_t* metadata;
+  float* trace_predictor;     // [batch, max_tokens, 640], or null: the joint's inputs at every emission
+  uint32_t* trace_frames;     // [batch, max_tokens]
   unsigned int* status;
   unsigned char* xchg;
   int batch, frames, max_tokens;
@@ -535,6 +537,8 @@ __device__ void projector(RSmem& s, const RParams& p) {
   if (live) {
     proj_at(p, w)[blockIdx.x * RCH + o] = acc;
     s.projv[w][o] = acc;
+    if (p.trace_predictor && s.win[w].count < p.max_tokens)
+      p.trace_predictor[((size_t)w * p.max_tokens + s.win[w].count) * RH + blockIdx.x * RCH + o] = acc;
   }
   // Joint input k = 5 cta + o of every window that takes a joint next (the
   // windows that did not update keep their last projector output).
@@ -837,6 +841,7 @@ __device__ void emit(RSmem& s, const RParams& p, int w, uint32_t tok, uint32_t f
       p.tokens[o] = tok;
       p.token_frames[o] = frame;
       p.token_durations[o] = dur;
+      if (p.trace_frames) p.trace_frames[o] = (uint32_t)c.joint_t;
     }
     ++c.count;
   } else {
@@ -1082,7 +1087,7 @@ __global__ void __launch_bounds__(RTHREADS, 1) tdt_resident_kernel(const RParams
 
 }  // namespace
 
-int launch_tdt_resident(const DeviceCtx& dev, const pk_tdt_desc& d, cudaStream_t stream) {
+int launch_tdt_resident(const DeviceCtx& dev, const pk_tdt_desc& d, const pk_tdt_trace& trace, cudaStream_t stream) {
   if (d.precision != PK_FP16 || d.batch > RMAXB || !dev.tdt_exchange || dev.sm_count < RG)
     return set_error(PK_E_SHAPE, "the resident decoder takes FP16 batches of at most %d windows on >= %d SMs", RMAXB,
                      RG);
@@ -1112,6 +1117,8 @@ int launch_tdt_resident(const DeviceCtx& dev, const pk_tdt_desc& d, cudaStream_t
   p.token_frames = d.token_frames;
   p.token_durations = d.token_durations;
   p.metadata = d.metadata;
+  p.trace_predictor = trace.predictor;
+  p.trace_frames = trace.joint_frames;
   p.status = dev.status;
   p.xchg = static_cast<unsigned char*>(dev.tdt_exchange);
   p.batch = d.batch;

@@ -24,8 +24,8 @@ import numpy as np
 from . import stitch as st
 from . import windows as wp
 from .encoder import ModelWeights, ParakeetEncoderGraph, derive_encoder_valid_length
-from .kernels import (Device, GpuTensor, ParakeetFbank, PersistentTdtDecoderKernel, RangeError,
-                      TDT_DECODER_TENSORS)
+from .kernels import (Device, GpuTensor, JointLogitsKernel, ParakeetFbank, PersistentTdtDecoderKernel, RangeError,
+                      TDT_DECODER_TENSORS, TokenScoresKernel)
 
 try:
     import torch
@@ -37,18 +37,37 @@ MAX_TOKENS_PER_WINDOW = 2048  # src/runtime/webgpu-engine.ts:84
 BATCH_CAPACITY = 40  # windows per batch, the reference's encoder capacity (src/webgpu/encoder.ts:68)
 
 
+TOKEN_COLUMNS, DURATION_COLUMNS = 1025, 5  # of the joint's 1032 outputs, padded by two
+
+
+@dataclass(frozen=True)
+class EmissionScores:
+    """What the joint says about each of a window's emissions (natural logarithms, f32)."""
+    token_log_probs: np.ndarray      # [n] of the emitted token, among the 1025 tokens (blank included)
+    duration_log_probs: np.ndarray   # [n] of the emitted duration, among the 5 durations
+    token_entropies: np.ndarray      # [n] of the token distribution
+    alternatives: np.ndarray         # int32 [n, k]: the k most probable tokens, best first
+    alternative_log_probs: np.ndarray  # [n, k]
+
+
 @dataclass(frozen=True)
 class WindowResult:
     """EngineWindowResult: one window's emissions in window-local frames."""
     tokens: tuple  # of stitch.EmittedToken
     overflow: bool
+    scores: EmissionScores | None = None  # from an engine created with `alternatives`
 
 
 class ParakeetEngine:
     def __init__(self, device: Device, package: dict, precision: str = "fp16", capacity: int = BATCH_CAPACITY,
-                 max_tokens: int = MAX_TOKENS_PER_WINDOW, keep_intermediates: bool = False):
+                 max_tokens: int = MAX_TOKENS_PER_WINDOW, keep_intermediates: bool = False,
+                 alternatives: int | None = None):
         """package: encoder + decoder tensors (name -> record), as produced by
-        the reference converter or ``synthetic.make_package`` + ``make_decoder``."""
+        the reference converter or ``synthetic.make_package`` + ``make_decoder``.
+        alternatives: when given, ``transcribe_windows`` scores every emission and
+        names its `alternatives` (0..32) most probable tokens."""
+        if alternatives is not None and not 0 <= alternatives <= 32:
+            raise RangeError(f"alternatives must be in [0, 32], got {alternatives}")
         self.device, self.precision, self.capacity, self.max_tokens = device, precision, capacity, max_tokens
         dec_names = set(TDT_DECODER_TENSORS)
         missing = sorted(dec_names - set(package))
@@ -79,26 +98,29 @@ class ParakeetEngine:
         for slot in self._slots:
             slot["pcm_np"] = slot["pcm"].numpy()
         self._copy_pool = ThreadPoolExecutor(max_workers=_staging_threads())
-        self._dispatch = self.decoder.create_dispatch(dict(
+        decode = dict(
             encoder_projected=self.graph.decoder_input(), encoded_lengths=self._control[1],
             decode_starts=self._control[2], decode_ends=self._control[3], flush_finals=self._control[4],
             tokens=self._tokens[0], token_frames=self._tokens[1], token_durations=self._tokens[2],
-            metadata=self._meta, batch_size=capacity, frames=188, max_tokens=max_tokens))
+            metadata=self._meta, batch_size=capacity, frames=188, max_tokens=max_tokens)
+        self._dispatch = self.decoder.create_dispatch(decode)
+        self._scorer = None if alternatives is None else _EmissionScorer(self, decode, alternatives)
         self.keep_intermediates = keep_intermediates
         self.last: dict = {}
 
     def transcribe_windows(self, windows: Sequence[tuple], stream=None) -> list[WindowResult]:
         """windows: (samples f32 [<= 240 000], WindowPlan) per window, 1..capacity."""
         out = []
-        for tok, fr, du, overflow in self._run_batch(windows, stream):
+        score = self._scorer is not None
+        for i, (tok, fr, du, overflow) in enumerate(self._run_batch(windows, stream, score)):
             out.append(WindowResult(tuple(map(st.EmittedToken._make, zip(tok.tolist(), fr.tolist(), du.tolist()))),
-                                    overflow))
+                                    overflow, self._scorer.window(i, len(tok)) if score else None))
         return out
 
-    def _run_batch(self, windows: Sequence[tuple], stream=None) -> list:
+    def _run_batch(self, windows: Sequence[tuple], stream=None, score: bool = False) -> list:
         """One batch through log-mel, encoder and decoder; per window its
         (token ids, frames, durations) arrays and overflow flag."""
-        out = self._collect(self._submit(windows, stream, 0))
+        out = self._collect(self._submit(windows, stream, 0, score=score))
         self._check_status()
         return out
 
@@ -109,10 +131,11 @@ class ParakeetEngine:
         in flight: reading the status word clears it."""
         self.device.status()
 
-    def _submit(self, windows: Sequence[tuple], stream, slot: int, decode: bool = True):
+    def _submit(self, windows: Sequence[tuple], stream, slot: int, decode: bool = True, score: bool = False):
         """Stages a batch in host slot `slot` and queues its copies and
         kernels on `stream` without waiting for them (without the decoder
-        and the token read-back when `decode` is False)."""
+        and the token read-back when `decode` is False; with the emissions'
+        scores when `score` is True)."""
         b = len(windows)
         if not 0 < b <= self.capacity:
             raise RangeError(f"Engine batch must contain 1-{self.capacity} windows")
@@ -148,7 +171,10 @@ class ParakeetEngine:
             self.fbank.compute_batch(self._pcm[:b], self._control[0, :b], out=self._features[:b], stream=stream)
             projected, _ = self.graph.encode(self._features[:b], lengths, stream=stream)
             if decode:
-                self._dispatch.encode(stream, active_batch_size=b)
+                if score:
+                    self._scorer.encode(b, stream)
+                else:
+                    self._dispatch.encode(stream, active_batch_size=b)
                 host["tokens"][:, :b].copy_(self._tokens[:, :b], non_blocking=True)
                 host["meta"].copy_(self._meta, non_blocking=True)
             host["done"].record(stream)
@@ -254,6 +280,72 @@ class ParakeetEngine:
         self._copy_pool.shutdown(wait=True)
         self.graph.destroy()
         self.weights.release()
+
+
+class _EmissionScorer:
+    """Decodes with a trace and scores every emission: the joint's logits of
+    the emissions alone (ragged, their number known on the device), then the
+    probabilities of the emitted tokens and durations, scattered to the places
+    of the tokens.  Everything runs on the batch's stream."""
+
+    def __init__(self, engine: ParakeetEngine, decode: dict, alternatives: int):
+        capacity, most, k = engine.capacity, engine.max_tokens, alternatives
+        cuda = engine._tokens.device
+        f32, i32 = dict(dtype=torch.float32, device=cuda), dict(dtype=torch.int32, device=cuda)
+        scalar = torch.float16 if engine.precision == "fp16" else torch.float32
+        self._k, self._most = k, most
+        self._predictor = torch.empty((capacity, most, 640), **f32)
+        self._frames = torch.zeros((capacity, most), **i32)
+        self._decode = engine.decoder.create_dispatch(dict(
+            decode, trace_predictor=self._predictor, trace_joint_frames=self._frames))
+        rows = capacity * most
+        self._logits = torch.empty((rows, TOKEN_COLUMNS + DURATION_COLUMNS + 2), dtype=scalar, device=cuda)
+        self._row_map, self._row_count = torch.zeros(rows, **i32), torch.zeros(1, **i32)
+        self._scores = torch.zeros((3, capacity, most), **f32)  # token and duration log probability, entropy
+        self._ids = torch.zeros((capacity, most, k), **i32)
+        self._id_scores = torch.zeros((capacity, most, k), **f32)
+        self._host = [torch.zeros(t.shape, dtype=t.dtype).pin_memory() for t in (self._scores, self._ids, self._id_scores)]
+        self._kernels = (JointLogitsKernel.create(engine.device, None, 0, engine.precision),
+                         TokenScoresKernel.create(engine.device, None, 0, engine.precision))
+        self._engine, self._steps = engine, {}
+
+    def _dispatches(self, batch: int) -> list:
+        """The scoring dispatches of a batch size (their shapes are fixed)."""
+        if batch not in self._steps:
+            eng, rows = self._engine, batch * self._most
+            w = eng._decoder_tensors
+            joint, scores = self._kernels
+            common = dict(logits=self._logits, rows=rows, row_stride=self._logits.shape[1], slots=rows,
+                          row_count=self._row_count, row_map=self._row_map)
+            token = dict(log_probs=self._scores[0], entropies=self._scores[2])
+            if self._k:
+                token.update(top_k=self._k, top_ids=self._ids, top_log_probs=self._id_scores)
+            self._steps[batch] = [
+                joint.create_dispatch(dict(
+                    label="emission-joint", encoder_projected=eng.graph.decoder_input(), predictor=self._predictor,
+                    joint_frames=self._frames, counts=eng._meta, weight=w["joint.head.weight"], bias=w["joint.head.bias"],
+                    logits=self._logits, row_map=self._row_map, row_count=self._row_count, batch_size=batch, frames=188,
+                    max_tokens=self._most, inner=640, columns=self._logits.shape[1])),
+                scores.create_dispatch(dict(common, label="token-scores", columns=TOKEN_COLUMNS, targets=eng._tokens[0],
+                                            **token)),
+                scores.create_dispatch(dict(common, label="duration-scores", columns=DURATION_COLUMNS,
+                                            first_column=TOKEN_COLUMNS, targets=eng._tokens[2],
+                                            log_probs=self._scores[1]))]
+        return self._steps[batch]
+
+    def encode(self, batch: int, stream) -> None:
+        self._decode.encode(stream, active_batch_size=batch)
+        for step in self._dispatches(batch):
+            step.encode(stream)
+        self._host[0][:, :batch].copy_(self._scores[:, :batch], non_blocking=True)
+        for host, dev in zip(self._host[1:], (self._ids, self._id_scores)):
+            host[:batch].copy_(dev[:batch], non_blocking=True)
+
+    def window(self, i: int, n: int) -> EmissionScores:
+        """The scores of window i's n emissions (once its batch is collected)."""
+        scores, ids, id_scores = (t.numpy() for t in self._host)
+        return EmissionScores(scores[0, i, :n].copy(), scores[1, i, :n].copy(), scores[2, i, :n].copy(),
+                              ids[i, :n].copy(), id_scores[i, :n].copy())
 
 
 def _staging_threads() -> int:

@@ -489,7 +489,9 @@ class PersistentTdtDecoderKernel:
     def create_dispatch(self, d: dict) -> _Dispatch:
         """d (TdtDecoderDescriptor, tdt-decoder.ts:54-82): label, encoder_projected,
         encoded_lengths, decode_starts, decode_ends, flush_finals, tokens, token_frames,
-        token_durations, metadata, batch_size, frames, max_tokens."""
+        token_durations, metadata, batch_size, frames, max_tokens; optionally
+        trace_predictor (f32 [batch, max_tokens, 640]) and trace_joint_frames (u32 [batch,
+        max_tokens]), which receive the joint's inputs at every emission."""
         for key in ("batch_size", "frames", "max_tokens"):
             v = d[key]
             if not isinstance(v, int) or v <= 0:
@@ -499,6 +501,11 @@ class PersistentTdtDecoderKernel:
         need = {"encoder_projected": b * t * 640 * esize, "encoded_lengths": b * 4, "decode_starts": b * 4,
                 "decode_ends": b * 4, "flush_finals": b * 4, "tokens": b * m * 4, "token_frames": b * m * 4,
                 "token_durations": b * m * 4, "metadata": b * 2 * 4}
+        traced = d.get("trace_predictor") is not None
+        if traced != (d.get("trace_joint_frames") is not None):
+            raise ParakeetError("A TDT trace needs trace_predictor and trace_joint_frames")
+        if traced:
+            need.update(trace_predictor=b * m * 640 * 4, trace_joint_frames=b * m * 4)
         for key, nbytes in need.items():
             buf = d[key]
             if buf.numel() * buf.element_size() < nbytes:
@@ -519,6 +526,11 @@ class PersistentTdtDecoderKernel:
                 w["decoder.decoder_projector.weight"], w["decoder.decoder_projector.bias"],
                 w["joint.head.weight"], w["joint.head.bias"], d["tokens"], d["token_frames"],
                 d["token_durations"], d["metadata"])])
+            if traced:
+                trace = _lib.TdtTrace(_ptr(d["trace_predictor"]), _ptr(d["trace_joint_frames"]))
+                _lib.call("pk_tdt_decode_traced", kernel.device.handle, ctypes.byref(desc), ctypes.byref(trace),
+                          _stream_handle(stream))
+                return
             _lib.call("pk_tdt_decode", kernel.device.handle, ctypes.byref(desc), _stream_handle(stream))
 
         disp.encode = encode

@@ -217,3 +217,17 @@ def test_int4_quantization_error(pk, precision, group):
     for bad in (0, 48, 96):
         with pytest.raises(ValueError, match="groups"):
             rp.quantize_int4(w, bad, precision)
+
+
+# ------------------------------------------------------------------ trace and engine
+
+def test_trace_and_alternatives_are_refused(pk):
+    lib = pk._lib
+    desc, trace = lib.TdtDesc(), lib.TdtTrace(P, None)
+    buf = _handle()
+    for tr in (None, ctypes.byref(trace)):
+        with pytest.raises(pk.PkError, match="trace"):
+            lib.call("pk_tdt_decode_traced", ctypes.cast(buf, ctypes.c_void_p), ctypes.byref(desc), tr, None)
+    for k in (-1, 33):
+        with pytest.raises(pk.kernels.RangeError, match="alternatives"):
+            pk.engine.ParakeetEngine(_FakeDevice(), {}, "fp16", alternatives=k)
