@@ -19,11 +19,10 @@
 // once with a running (m, s, u) per thread.
 //
 // Alternatives cost nothing while the row is read: a lane knows its largest
-// value, and lane maxima bound the K-th best value from below: where every one
-// of the row's w warps has ceil(K / w) lanes that reach a value, K columns do.
-// Few values reach that bound (about K times the w-th harmonic number); they
-// go to a pool in shared memory and each counts how many of the pool beat it:
-// its rank.  A pool that
+// value, and the K-th largest of any maxima of parts of the row bounds the K-th
+// best value from below.  Few values reach that bound (of 16 half warps, 11 for
+// K = 8); they go to a pool in shared memory and each counts how many of the
+// pool beat it: its rank.  A pool that
 // overflows (a row of many equal values) is replaced by sorted lists, one per
 // warp, into which candidates are inserted one at a time.  Where fewer than K
 // columns are left by a mask, the lowest masked ids fill the places.
@@ -81,6 +80,7 @@ struct TsSmem {
   TsStat cstat[TS_CLUSTER];
   alignas(16) uint32_t lane_max[TS_WARPS][32];
   uint32_t bound[TS_WARPS];              // per warp
+  uint32_t half_max[2 * TS_WARPS];
   int count[TS_WARPS];                   // per row: candidates
 };
 
@@ -300,12 +300,28 @@ __device__ __forceinline__ void ts_row_sync(int group, int wpr) {
 }
 
 // A value (ordered bits) that at least k of the row's columns in this CTA
-// reach, where k are unmasked: the least of the warps' j-th largest lane
-// maxima, j = ceil(k / wpr).  More than -inf: no masked value is a candidate.
+// reach, where k are unmasked.  While the row has k half warps, the k-th largest
+// of their maxima; else the least of the warps' j-th largest lane maxima,
+// j = ceil(k / wpr).  More than -inf: no masked value is a candidate.
 __device__ __forceinline__ uint32_t ts_bound(TsSmem& sm, uint32_t mine, int group, int wpr, int k) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int j = (k + wpr - 1) / wpr;
   uint32_t bound;
+  if (wpr > 1 && k <= 2 * wpr) {
+    uint32_t top = mine;  // of the half warp
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((lane & 15) == 0) sm.half_max[2 * warp + (lane >> 4)] = top;
+    ts_row_sync(group, wpr);
+    const uint32_t* of = sm.half_max + 2 * group * wpr;
+    const uint32_t v = lane < 2 * wpr ? of[lane] : 0;
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < 2 * TS_WARPS; ++i)
+      if (i < 2 * wpr) above += of[i] > v;
+    bound = __reduce_min_sync(0xffffffffu, lane < 2 * wpr && above < k ? v : 0xffffffffu);
+    return max(bound, TS_MASKED + 1);
+  }
+  const int j = (k + wpr - 1) / wpr;
   if (j == 1) {
     bound = __reduce_max_sync(0xffffffffu, mine);
   } else {
@@ -449,15 +465,12 @@ __global__ void __launch_bounds__(TS_THREADS, sizeof(T) == 2 && NV > 0 ? (NV == 
       }
       tile.sums(m, ma, mb, s2, u2);
     };
-    // The next tile is on its way while one is summed.
-    TsTile<T, TS_UNR> a, b;
-    if (first < vectors) a.load(base, skew, columns, first, lane, 32, vectors);
-    for (int v = first; v < vectors; v += 2 * step) {
-      if (v + step < vectors) b.load(base, skew, columns, v + step, lane, 32, vectors);
-      take(a);
-      if (v + step >= vectors) break;
-      if (v + 2 * step < vectors) a.load(base, skew, columns, v + 2 * step, lane, 32, vectors);
-      take(b);
+    // The warps of four CTAs an SM cover each other's loads (a second tile in
+    // registers, loaded ahead, was 7% slower: fewer warps, more moves).
+    TsTile<T, TS_UNR> tile;
+    for (int v = first; v < vectors; v += step) {
+      tile.load(base, skew, columns, v, lane, 32, vectors);
+      take(tile);
     }
     // The lanes' sums, brought to the warp's maximum.
     st = TsStat{ts_value(__reduce_max_sync(0xffffffffu, ts_ordered(m))), s2.x + s2.y, u2.x + u2.y};

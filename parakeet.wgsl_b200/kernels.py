@@ -676,6 +676,13 @@ class SubsamplingTimeMaskKernel:
 # the layer's shape (create -> create_dispatch -> encode -> destroy).  A
 # dispatch's pointers and sizes are fixed at creation, so encode is one C call.
 
+def _current_stream(ordinal: int) -> int:
+    """The handle of device `ordinal`'s current stream.  Decode steps make this call per operator; the
+    raw accessor costs a tenth of building a torch.cuda.Stream."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(ordinal) if raw is not None else torch.cuda.current_stream(ordinal).cuda_stream
+
+
 class _FixedDispatch(_Dispatch):
     """A dispatch whose descriptor never changes; keeps its buffers alive."""
 
@@ -689,7 +696,7 @@ class _FixedDispatch(_Dispatch):
         if self._destroyed or self._device.handle is None:
             raise ParakeetError(f"{self.label} was destroyed")
         if stream is None:
-            stream = torch.cuda.current_stream(self._device.ordinal).cuda_stream
+            stream = _current_stream(self._device.ordinal)
         else:
             stream = _stream_handle(stream)
         status = self._entry(self._device.handle, self._ref, stream)
