@@ -52,9 +52,13 @@ constexpr int I4_COLS = 32;       // columns of one pass, at most (more rows: th
 constexpr int I4_CLUSTER = 8;     // CTAs that share the inputs, at most
 constexpr int I4_SMEM = 220 * 1024;
 
-// Warps per CTA (registers: 72, 96, 128 a thread) and tiles in flight per warp.
-__host__ __device__ constexpr int i4_warps(int nt) { return nt == 1 ? 28 : nt == 2 ? 20 : 16; }
-constexpr int I4_DEPTH = 3;
+// Warps per CTA (registers: 72, 128, 128 a thread), tiles of outputs a warp takes
+// at a time and tiles in flight per warp, by column tiles.  With two output
+// tiles a column leaves shared memory half as often: 16x4096x65536 f16 53 -> 48
+// us; with 32 columns their sums leave room for 12 warps alone, 86 -> 92 us.
+__host__ __device__ constexpr int i4_warps(int nt) { return nt == 1 ? 28 : 16; }
+__host__ __device__ constexpr int i4_mt(int nt) { return nt == 2 ? 2 : 1; }
+__host__ __device__ constexpr int i4_depth(int nt) { return nt == 2 ? 2 : 3; }
 
 struct I4Params {
   const void* a;
@@ -227,14 +231,15 @@ __device__ __forceinline__ void i4_stage(const I4Params& p, unsigned char* xs, f
   }
 }
 
-// NT tiles of 8 columns, GB blocks of 32 inputs per scale within a tile (1, 2,
-// or 4: groups of whole tiles).
+// NT tiles of 8 columns, MT tiles of 16 outputs a warp at a time, GB blocks of
+// 32 inputs per scale within a tile (1, 2, or 4: groups of whole tiles).
 template <typename T, int NT, int GB>
 __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I4Params p) {
+  constexpr int MT = i4_mt(NT);
   extern __shared__ __align__(128) unsigned char i4_smem[];
   constexpr int PARTS = sizeof(T) == 2 ? 1 : 2;  // columns per row
   constexpr int SPT = 4 / GB;                    // scales per tile and output
-  constexpr int DEPTH = I4_DEPTH;
+  constexpr int DEPTH = i4_depth(NT);
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // the same in all lanes, and known to be
   const int g = lane >> 2, t = lane & 3;
@@ -244,7 +249,8 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
   const int rows = min(p.rows - row0, p.rows_per_pass);
   const int cols = rows * PARTS;
   const int mtiles = (p.columns + 15) / 16;
-  const int walk = (int)gridDim.x / p.cluster * p.wm;  // tiles of outputs between a warp's
+  const int mgroups = (mtiles + MT - 1) / MT;           // a warp's outputs, MT tiles each
+  const int walk = (int)gridDim.x / p.cluster * p.wm;  // groups of outputs between a warp's
   const int k0 = rank * p.ktiles_cta;                  // this CTA's tiles of inputs
   const int ktiles = max(0, min(p.ktiles_cta, p.ktiles - k0));
   unsigned char* xs = i4_smem;
@@ -253,8 +259,8 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
   float* xscale = addend + (size_t)p.ktiles_cta * SPT * NT * 16;
 
   struct Slot {
-    uint4 code[2];
-    T scale[2];  // of the tile's scale t % SPT; lanes exchange them when they are used
+    uint4 code[MT][2];
+    T scale[MT][2];  // of the tile's scale t % SPT; lanes exchange them when they are used
   };
   Slot ring[DEPTH];
   // What is loaded next: this warp's tile `lk` of inputs (of the CTA's) for
@@ -263,30 +269,38 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
   const int rounds = (p.ktiles_cta + p.wk * DEPTH - 1) / (p.wk * DEPTH);
   const int round_end = wk + rounds * DEPTH * p.wk;
   const int first = (int)blockIdx.x / p.cluster * p.wm + wm;
-  int lm = first, lk = wk, lend = first < mtiles ? ktiles : 0;
-  const uint4* lcode;
-  const T* lscale;
+  int lm = first, lk = wk, lend = first < mgroups ? ktiles : 0;
+  const uint4* lcode[MT];
+  const T* lscale[MT];
   auto aim = [&]() {
-    lcode = p.codes + ((size_t)lm * p.ktiles + k0 + lk) * 64 + lane;
-    lscale = static_cast<const T*>(p.scales) + (size_t)lm * p.groups * 16 + g;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int mt = min(lm * MT + m, mtiles - 1);
+      lcode[m] = p.codes + ((size_t)mt * p.ktiles + k0 + lk) * 64 + lane;
+      lscale[m] = static_cast<const T*>(p.scales) + (size_t)mt * p.groups * 16 + g;
+    }
   };
   aim();
   auto load = [&](Slot& s) {
     if (lk < lend) {
-      s.code[0] = i4_load(lcode);
-      s.code[1] = i4_load(lcode + 32);
       const int kt = k0 + lk;
       const int gi = GB == 4 ? (p.group_inv ? (int)__umulhi((uint32_t)kt, p.group_inv) : kt)
                              : min(kt * SPT + (t & (SPT - 1)), p.groups - 1);
-      s.scale[0] = __ldg(lscale + gi * 16);
-      s.scale[1] = __ldg(lscale + gi * 16 + 8);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        s.code[m][0] = i4_load(lcode[m]);
+        s.code[m][1] = i4_load(lcode[m] + 32);
+        s.scale[m][0] = __ldg(lscale[m] + gi * 16);
+        s.scale[m][1] = __ldg(lscale[m] + gi * 16 + 8);
+      }
     }
     lk += p.wk;
-    lcode += p.wk * 64;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) lcode[m] += p.wk * 64;
     if (lk == round_end) {
       lk = wk;
       lm += walk;
-      if (lm >= mtiles) lend = 0;
+      if (lm >= mgroups) lend = 0;
       aim();
     }
   };
@@ -305,59 +319,71 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
     xsc[n] = smem_addr(xscale + min(n * 4 + t, rows - 1) * p.ktiles_cta);  // FP32: columns 2 t and 2 t + 1 are one row
   }
   const uint32_t xadd = smem_addr(addend) + t * 16;
-  const int M = p.wm * 16;
+  const int M = p.wm * MT * 16;
   constexpr int PC = NT * 8;
   float* part = reinterpret_cast<float*>(i4_smem + p.part_offset);  // [wk][column][output]
   float* sums = part + (size_t)p.wk * PC * (M + 4);                 // cluster: [parity][row][output]
-  const int pm = tid % M, pr = tid / M;  // the output and first row that this thread joins (2 wk threads per output)
+  const int pm = tid % M, pr = tid / M;  // the output and first row that this thread joins
+  const int rstep = (int)blockDim.x / M;   // threads per output
   int parity = 0;
-  for (int m0 = (int)blockIdx.x / p.cluster * p.wm; m0 < mtiles; m0 += walk, parity ^= 1) {
-    float total[NT][4] = {};
+  for (int m0 = (int)blockIdx.x / p.cluster * p.wm; m0 < mgroups; m0 += walk, parity ^= 1) {
+    float total[MT][NT][4] = {};
     for (int r = 0; r < rounds; ++r) {
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
         const int kl = wk + (r * DEPTH + d) * p.wk;
         Slot& s = ring[d];
-        if (kl < ktiles && m0 + wm < mtiles) {
+        if (kl < ktiles && m0 + wm < mgroups) {
 #pragma unroll
           for (int b = 0; b < SPT; ++b) {
-            float acc[NT][4];
+            float acc[MT][NT][4];
 #pragma unroll
             for (int i = b * GB; i < (b + 1) * GB; ++i) {
               uint4 x[NT];
 #pragma unroll
-              for (int n = 0; n < NT; ++n)
-                x[n] = i4_lds(xcol[n] + kl * (I4_KT * 2) + i * 64);
-              uint32_t w0[4], w1[4];
-              i4_expand((&s.code[0].x)[i], w0);
-              i4_expand((&s.code[1].x)[i], w1);
+              for (int n = 0; n < NT; ++n) x[n] = i4_lds(xcol[n] + kl * (I4_KT * 2) + i * 64);
+              uint32_t w0[MT][4], w1[MT][4];
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                i4_expand((&s.code[m][0].x)[i], w0[m]);
+                i4_expand((&s.code[m][1].x)[i], w1[m]);
+              }
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                if (i == b * GB)
-                  i4_mma_first(acc[n], w0[0], w1[0], w0[1], w1[1], x[n].x, x[n].y,
-                               i4_lds(xadd + (kl * SPT + b) * (NT * 64) + n * 64));
-                else
-                  i4_mma(acc[n], w0[0], w1[0], w0[1], w1[1], x[n].x, x[n].y);
-                i4_mma(acc[n], w0[2], w1[2], w0[3], w1[3], x[n].z, x[n].w);
+                if (i == b * GB) {
+                  const uint4 c = i4_lds(xadd + (kl * SPT + b) * (NT * 64) + n * 64);
+#pragma unroll
+                  for (int m = 0; m < MT; ++m) i4_mma_first(acc[m][n], w0[m][0], w1[m][0], w0[m][1], w1[m][1], x[n].x, x[n].y, c);
+                } else {
+#pragma unroll
+                  for (int m = 0; m < MT; ++m) i4_mma(acc[m][n], w0[m][0], w1[m][0], w0[m][1], w1[m][1], x[n].x, x[n].y);
+                }
+#pragma unroll
+                for (int m = 0; m < MT; ++m) i4_mma(acc[m][n], w0[m][2], w1[m][2], w0[m][3], w1[m][3], x[n].z, x[n].w);
               }
             }
-            float s0 = (float)s.scale[0], s1 = (float)s.scale[1];
-            if constexpr (SPT > 1) {
-              s0 = __shfl_sync(0xffffffffu, s0, (lane & ~3) | b);
-              s1 = __shfl_sync(0xffffffffu, s1, (lane & ~3) | b);
+            float s0[MT], s1[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              s0[m] = (float)s.scale[m][0];
+              s1[m] = (float)s.scale[m][1];
+              if constexpr (SPT > 1) {
+                s0[m] = __shfl_sync(0xffffffffu, s0[m], (lane & ~3) | b);
+                s1[m] = __shfl_sync(0xffffffffu, s1[m], (lane & ~3) | b);
+              }
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              float f0 = s0, f1 = s1;
-              if constexpr (PARTS == 2) {
-                const float f = i4_lds_f32(xsc[n] + 4 * kl);
-                f0 *= f;
-                f1 *= f;
+              float f = 1.0f;
+              if constexpr (PARTS == 2) f = i4_lds_f32(xsc[n] + 4 * kl);
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                const float f0 = PARTS == 2 ? s0[m] * f : s0[m], f1 = PARTS == 2 ? s1[m] * f : s1[m];
+                total[m][n][0] = fmaf(f0, acc[m][n][0], total[m][n][0]);
+                total[m][n][1] = fmaf(f0, acc[m][n][1], total[m][n][1]);
+                total[m][n][2] = fmaf(f1, acc[m][n][2], total[m][n][2]);
+                total[m][n][3] = fmaf(f1, acc[m][n][3], total[m][n][3]);
               }
-              total[n][0] = fmaf(f0, acc[n][0], total[n][0]);
-              total[n][1] = fmaf(f0, acc[n][1], total[n][1]);
-              total[n][2] = fmaf(f1, acc[n][2], total[n][2]);
-              total[n][3] = fmaf(f1, acc[n][3], total[n][3]);
             }
           }
         }
@@ -365,10 +391,12 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
       }
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        part[((size_t)wk * PC + n * 8 + 2 * t + (e & 1)) * (M + 4) + wm * 16 + g + 8 * (e >> 1)] = total[n][e];
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          part[((size_t)wk * PC + n * 8 + 2 * t + (e & 1)) * (M + 4) + (wm * MT + m) * 16 + g + 8 * (e >> 1)] = total[m][n][e];
     __syncthreads();
     auto finish = [&](int r, int n, float v) {
       if (n >= p.columns) return;
@@ -379,14 +407,14 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
       if (p.residual) v = fmaf(p.residual_scale, v, (float)static_cast<const T*>(p.residual)[at]);
       static_cast<T*>(p.c)[at] = (T)v;
     };
-    for (int r = pr; r < rows; r += 2 * p.wk) {
+    for (int r = pr; r < rows; r += rstep) {
       float v = 0.0f;
       const float* src = part + (size_t)r * PARTS * (M + 4) + pm;
       for (int w = 0; w < p.wk; ++w, src += PC * (M + 4)) {
         v += src[0];
         if constexpr (PARTS == 2) v += src[M + 4];
       }
-      if (p.cluster == 1) finish(r, m0 * 16 + pm, v);
+      if (p.cluster == 1) finish(r, m0 * MT * 16 + pm, v);
       else sums[(size_t)(parity * rows + r) * M + pm] = v;
     }
     __syncthreads();  // the parts are read (and the sums written)
@@ -394,7 +422,7 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
       // Each CTA finishes its share of the rows.  The sums of this parity are
       // written again two tiles on, behind the next tile's barrier.
       cluster_sync();
-      for (int r = pr * p.cluster + rank; r < rows; r += 2 * p.wk * p.cluster) {
+      for (int r = pr * p.cluster + rank; r < rows; r += rstep * p.cluster) {
         const uint32_t at = smem_addr(sums + (size_t)(parity * rows + r) * M + pm);
         float u[I4_CLUSTER];
 #pragma unroll
@@ -404,7 +432,7 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
 #pragma unroll
         for (int c = 0; c < I4_CLUSTER; ++c)
           if (c < p.cluster) v += u[c];
-        finish(r, m0 * 16 + pm, v);
+        finish(r, m0 * MT * 16 + pm, v);
       }
     }
   }
@@ -483,33 +511,35 @@ int launch_typed(const DeviceCtx& dev, I4Params p, int group, cudaStream_t strea
   constexpr int PARTS = sizeof(T) == 2 ? 1 : 2;
   const int mtiles = (p.columns + 15) / 16;
   int cols = std::min(p.rows * PARTS, I4_COLS);
-  int nt = 0, smem = 0, clusters = 0;
+  int nt = 0, smem = 0, clusters = 0, mgroups = 0;
   // Columns per pass, then CTAs per cluster: the least that fit.
   for (;; cols = std::max(PARTS, cols / 2 / PARTS * PARTS)) {
     p.rows_per_pass = cols / PARTS;
     nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-    const int warps = i4_warps(nt);
+    const int mt = i4_mt(nt), warps = i4_warps(nt);
+    mgroups = (mtiles + mt - 1) / mt;
     for (p.cluster = 1; p.cluster <= I4_CLUSTER; p.cluster *= 2) {
       // Few outputs: the inputs over more SMs, while each has a tile for every warp of 4.
-      if (mtiles * p.cluster * 2 <= dev.sm_count && p.cluster < I4_CLUSTER && p.ktiles >= p.cluster * 2 * 4) continue;
+      if (mgroups * p.cluster * 2 <= dev.sm_count && p.cluster < I4_CLUSTER && p.ktiles >= p.cluster * 2 * 4) continue;
       p.ktiles_cta = (p.ktiles + p.cluster - 1) / p.cluster;
       const int st = i4_clusters(dev, p.cluster, &clusters);
       if (st != PK_OK) return st;
-      const int q = (mtiles + clusters - 1) / clusters;  // output tiles of a cluster
+      const int q = (mgroups + clusters - 1) / clusters;  // groups of outputs of a cluster
       const int turns = (q + warps - 1) / warps;
       p.wm = (q + turns - 1) / turns;
       p.wk = std::max(1, std::min(p.ktiles_cta, warps / p.wm));
       const int spt = group == 32 ? 4 : group == 64 ? 2 : 1;
       p.part_offset = cols * i4_col_bytes(p.ktiles_cta) + p.ktiles_cta * spt * nt * 64;
       p.part_offset = (p.part_offset + (PARTS == 2 ? p.rows_per_pass * p.ktiles_cta * 4 : 0) + 127) / 128 * 128;
-      smem = p.part_offset + p.wk * nt * 8 * (p.wm * 16 + 4) * 4 + (p.cluster > 1 ? 2 * p.rows_per_pass * p.wm * 16 * 4 : 0);
+      smem = p.part_offset + p.wk * nt * 8 * (p.wm * mt * 16 + 4) * 4 +
+             (p.cluster > 1 ? 2 * p.rows_per_pass * p.wm * mt * 16 * 4 : 0);
       if (smem <= I4_SMEM) break;
     }
     if (p.cluster <= I4_CLUSTER || cols == PARTS) break;
   }
   if (smem > I4_SMEM) return set_error(PK_E_SHAPE, "int4 products of K=%d do not fit shared memory", p.inner);
   const int passes = (p.rows + p.rows_per_pass - 1) / p.rows_per_pass;
-  clusters = std::min(clusters, (mtiles + p.wm - 1) / p.wm);
+  clusters = std::min(clusters, (mgroups + p.wm - 1) / p.wm);
   const dim3 grid((unsigned)(clusters * p.cluster), (unsigned)passes);
   if (nt == 1) return launch_group<T, 1>(p, group, grid, smem, stream);
   if (nt == 2) return launch_group<T, 2>(p, group, grid, smem, stream);
