@@ -243,7 +243,9 @@ int pk_tdt_decode_traced(pk_device* device, const pk_tdt_desc* desc, const pk_td
  * counterparts in the reference, which returns token ids alone.  No entry
  * point here holds a workspace: calls on different streams may overlap, and
  * captured graphs may run side by side.  Each leaves the calling thread's
- * current device as it was.
+ * current device as it was.  Buffers are aligned to their elements, or to what
+ * their field says; an output that overlaps another buffer of the call is
+ * refused, but for the exact aliases that are named.
  *
  * Token scores: for every row of logits x [columns], with the softmax p:
  *   log_probs   log p[target]      log_sums   log sum exp x
@@ -261,7 +263,7 @@ typedef struct pk_token_scores_desc {
   const void* logits;        /* device; element-aligned */
   const uint32_t* targets;   /* device u32 [slots] or NULL */
   const uint32_t* row_count; /* device u32 [1] or NULL: rows at and behind it are left out */
-  const uint32_t* row_map;   /* device u32 [rows] or NULL: row r takes targets and outputs at slot row_map[r] */
+  const uint32_t* row_map;   /* device u32 [rows] or NULL: row r takes targets and outputs at slot row_map[r], each its own */
   int64_t slots;             /* entries of targets and outputs; rows whose slot is outside are left out */
   float* log_probs;          /* device f32 [slots] */
   float* log_sums;
@@ -302,7 +304,8 @@ int pk_residual_norm(pk_device* device, const pk_residual_norm_desc* desc, pk_st
 
 /* A few rows times a matrix held in 4 bits, the decode form of the palette
  * GEMM: C = epilogue(A . W), W[k, n] = (code[k, n] - 8) * scale[k / group, n].
- * The scale multiplies the group's f32 sum.  Epilogue as in pk_gemm_desc; bias
+ * The scale multiplies the group's f32 sum; an infinite or NaN input adds its
+ * product as the formula does.  Epilogue as in pk_gemm_desc; bias
  * and residual are exclusive.  Codes lie in tiles of 16 outputs x 128 inputs
  * ("n16-k128-lane-major-int4-u32"): u32 [ceil(N / 16)][ceil(K / 128)][2][32][4],
  * where word i of lane l in half h holds, lowest bits first, the codes of
@@ -332,7 +335,8 @@ int pk_int4_gemv(pk_device* device, const pk_int4_gemv_desc* desc, pk_stream str
  * for u < min(counts[w], max_tokens), rows in order of (w, u); FP16 rounds
  * hidden to f16, as the decoder does.  row_map[r] = w * max_tokens + u and
  * row_count are what pk_token_scores takes.  Rows behind the last are left as
- * they are.  Frames >= frames are read as frames - 1. */
+ * they are.  Frames >= frames are read as frames - 1.  FP32 products are sums of three
+ * in shorter parts: an infinite hidden value or weight makes NaN. */
 typedef struct pk_joint_logits_desc {
   int precision;                 /* PK_FP16: encoder, weight, logits f16; PK_FP32: f32 */
   int batch, frames, max_tokens;

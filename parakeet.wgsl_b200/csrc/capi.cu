@@ -13,6 +13,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <set>
 #include <string>
@@ -102,6 +103,32 @@ struct DeviceScope {
 };
 
 static inline bool misaligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
+// A buffer of a call, for its checks of alignment and overlap.
+struct Span {
+  const char* name;
+  const void* p;
+  int64_t bytes;
+  int align;
+};
+
+// Outputs must be aligned and overlap neither inputs nor each other.
+static int check_spans(const char* what, std::initializer_list<Span> outs, std::initializer_list<Span> ins) {
+  auto apart = [](const Span& a, const Span& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return !x || !y || x + (uintptr_t)a.bytes <= y || y + (uintptr_t)b.bytes <= x;
+  };
+  for (const auto* list : {&outs, &ins})
+    for (const Span& s : *list)
+      if (misaligned(s.p, (uintptr_t)s.align)) return set_error(PK_E_LAYOUT, "%s: %s must be %d-byte aligned", what, s.name, s.align);
+  for (const Span* o = outs.begin(); o != outs.end(); ++o) {
+    for (const Span* q = outs.begin(); q != o; ++q)
+      if (!apart(*o, *q)) return set_error(PK_E_INVALID, "%s: %s overlaps %s", what, o->name, q->name);
+    for (const Span& i : ins)
+      if (!apart(*o, i)) return set_error(PK_E_INVALID, "%s: %s overlaps %s", what, o->name, i.name);
+  }
+  return PK_OK;
+}
 
 }  // namespace pk
 
@@ -323,6 +350,8 @@ int pk_tdt_decode(pk_device* device, const pk_tdt_desc* d, pk_stream stream) {
 
 int pk_tdt_decode_traced(pk_device* device, const pk_tdt_desc* d, const pk_tdt_trace* trace, pk_stream stream) {
   if (!trace || !trace->predictor || !trace->joint_frames) return set_error(PK_E_INVALID, "TDT trace pointer is null");
+  if (misaligned(trace->predictor, 16) || misaligned(trace->joint_frames, 4))
+    return set_error(PK_E_LAYOUT, "the TDT trace's predictor must be 16-byte, its frames 4-byte aligned");
   return tdt_decode(device, d, *trace, stream);
 }
 
@@ -389,6 +418,8 @@ int pk_token_scores(pk_device* device, const pk_token_scores_desc* d, pk_stream 
     return set_error(PK_E_SHAPE, "token scores take 1..2^30 rows and columns");
   if (d->row_stride < d->columns) return set_error(PK_E_SHAPE, "row stride %lld is below the %lld columns",
                                                    (long long)d->row_stride, (long long)d->columns);
+  if (d->row_stride > ((int64_t)1 << 60) / d->rows || d->slots > (int64_t)1 << 32)
+    return set_error(PK_E_SHAPE, "token scores take at most 2^60 elements and 2^32 slots");
   if (d->top_k < 0 || d->top_k > 32 || d->top_k > d->columns)
     return set_error(PK_E_SHAPE, "top_k must be in [0, 32] and at most the columns, got %d", d->top_k);
   if (d->slots < (d->row_map ? 1 : d->rows)) return set_error(PK_E_SHAPE, "outputs hold %lld of %lld rows",
@@ -396,7 +427,19 @@ int pk_token_scores(pk_device* device, const pk_token_scores_desc* d, pk_stream 
   if (d->log_probs && !d->targets) return set_error(PK_E_INVALID, "log probabilities need target ids");
   if (!d->log_probs && !d->log_sums && !d->entropies && !d->top_ids && !d->top_log_probs)
     return set_error(PK_E_INVALID, "token scores without an output");
-  if (misaligned(d->logits, d->precision == PK_FP16 ? 2 : 4)) return set_error(PK_E_LAYOUT, "logits are not element-aligned");
+  const int es = d->precision == PK_FP16 ? 2 : 4;
+  const int64_t each = 4 * d->slots, best = each * d->top_k;
+  const int st = check_spans("token scores",
+                             {{"log_probs", d->log_probs, each, 4},
+                              {"log_sums", d->log_sums, each, 4},
+                              {"entropies", d->entropies, each, 4},
+                              {"top_ids", d->top_ids, best, 4},
+                              {"top_log_probs", d->top_log_probs, best, 4}},
+                             {{"logits", d->logits, ((d->rows - 1) * d->row_stride + d->columns) * es, es},
+                              {"targets", d->targets, each, 4},
+                              {"row_count", d->row_count, 4, 4},
+                              {"row_map", d->row_map, 4 * d->rows, 4}});
+  if (st != PK_OK) return st;
   DeviceScope scope(device->ctx);
   if (scope.status != PK_OK) return scope.status;
   return launch_token_scores(device->ctx, *d, as_stream(stream));
@@ -432,6 +475,15 @@ int pk_residual_norm(pk_device* device, const pk_residual_norm_desc* d, pk_strea
       if (o && i && a != b && a < b + bytes && b < a + bytes)
         return set_error(PK_E_INVALID, "residual norm buffers overlap without being the same");
     }
+  const int64_t row = 4 * d->channels, gates = d->gate_rows ? (d->rows - 1) / d->gate_rows + 1 : 1;
+  const int st = check_spans("residual norm",
+                             {{"output", d->output, (int64_t)bytes, (int)es}, {"normalized", d->normalized, (int64_t)bytes, (int)es}},
+                             {{"post_gamma", d->post_gamma, row, 4},
+                              {"post_beta", d->post_beta, row, 4},
+                              {"pre_gamma", d->pre_gamma, row, 4},
+                              {"pre_beta", d->pre_beta, row, 4},
+                              {"gate", d->gate, gates * row, 4}});
+  if (st != PK_OK) return st;
   DeviceScope scope(device->ctx);
   if (scope.status != PK_OK) return scope.status;
   return launch_residual_norm(device->ctx, *d, as_stream(stream));
@@ -449,7 +501,18 @@ int pk_int4_gemv(pk_device* device, const pk_int4_gemv_desc* d, pk_stream stream
                      (long long)d->group, (long long)d->inner);
   if (d->activation < PK_ACT_NONE || d->activation > PK_ACT_RELU) return set_error(PK_E_INVALID, "unknown activation %d", d->activation);
   if (d->bias && d->residual) return set_error(PK_E_SIGNATURE, "cannot fuse bias and residual together");
-  if (misaligned(d->a, 16) || misaligned(d->codes, 16)) return set_error(PK_E_LAYOUT, "int4 rows and codes must be 16-byte aligned");
+  const int es = d->precision == PK_FP16 ? 2 : 4;
+  const int64_t tiles = (d->columns + 15) / 16;
+  const Span c{"c", d->c, d->rows * d->columns * es, es};
+  // A residual that is C itself is read by the thread that writes its place.
+  const Span residual{"residual", d->residual == d->c ? nullptr : d->residual, c.bytes, es};
+  const int st = check_spans("int4 product", {c},
+                             {{"a", d->a, d->rows * d->inner * es, 16},
+                              {"codes", d->codes, tiles * ((d->inner + 127) / 128) * 1024, 16},
+                              {"scales", d->scales, tiles * (d->inner / d->group) * 16 * es, es},
+                              {"bias", d->bias, 4 * d->columns, 4},
+                              residual});
+  if (st != PK_OK) return st;
   DeviceScope scope(device->ctx);
   if (scope.status != PK_OK) return scope.status;
   return launch_int4_gemv(device->ctx, *d, as_stream(stream));
@@ -468,9 +531,19 @@ int pk_joint_logits(pk_device* device, const pk_joint_logits_desc* d, pk_stream 
       d->columns > (1 << 20))
     return set_error(PK_E_SHAPE, "Unsupported joint shape: K=%lld N=%lld (needs K%%32==0, N%%8==0)", (long long)d->inner,
                      (long long)d->columns);
-  const void* aligned16[] = {d->encoder_projected, d->predictor, d->weight, d->logits, d->bias};
-  for (const void* q : aligned16)
-    if (misaligned(q, 16)) return set_error(PK_E_LAYOUT, "joint operands must be 16-byte aligned");
+  const int es = d->precision == PK_FP16 ? 2 : 4;
+  const int64_t rows = (int64_t)d->batch * d->max_tokens;
+  const int st = check_spans("joint",
+                             {{"logits", d->logits, rows * d->columns * es, 16},
+                              {"row_map", d->row_map, 4 * rows, 4},
+                              {"row_count", d->row_count, 4, 4}},
+                             {{"encoder_projected", d->encoder_projected, (int64_t)d->batch * d->frames * d->inner * es, 16},
+                              {"predictor", d->predictor, 4 * rows * d->inner, 16},
+                              {"joint_frames", d->joint_frames, 4 * rows, 4},
+                              {"counts", d->counts, (int64_t)4 * d->batch, 4},
+                              {"weight", d->weight, d->inner * d->columns * es, 16},
+                              {"bias", d->bias, 4 * d->columns, 16}});
+  if (st != PK_OK) return st;
   DeviceScope scope(device->ctx);
   if (scope.status != PK_OK) return scope.status;
   return launch_joint_logits(device->ctx, *d, as_stream(stream));

@@ -27,7 +27,8 @@
 // rounded.  FP32 rows are two f16 columns each, the leading 11 bits and the
 // next 11, after a power-of-two scale per row and 128 inputs that brings the
 // largest to [2^14, 2^15): 22 bits of every input, where the sum's own rounding
-// is 24.
+// is 24.  An infinite or NaN input is laid out as 0 and its row marked; the
+// thread that joins such a row's sum adds those products itself, from A.
 //
 // One CTA per SM walks the output tiles; A's rows are laid out in its shared
 // memory once.  Its warps split outputs (wm) and inputs (wk), so that the
@@ -143,11 +144,30 @@ __device__ __forceinline__ float* i4_addend(float* base, int block, int col) {
   return base + (size_t)(block * NT * 4 + (col >> 1)) * 4 + (col & 1);
 }
 
+// The products of row r's infinite and NaN inputs of tiles [kt0, kt0 + tiles) with output n.
+template <typename T>
+__device__ float i4_special(const I4Params& p, int r, int n, int kt0, int tiles) {
+  const T* a = static_cast<const T*>(p.a) + (size_t)r * p.inner;
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(p.codes) + ((size_t)(n >> 4) * p.ktiles) * 256;
+  const T* scales = static_cast<const T*>(p.scales) + (size_t)(n >> 4) * p.groups * 16 + (n & 15);
+  const int group = p.inner / p.groups;
+  const int end = min((kt0 + tiles) * I4_KT, p.inner);
+  float v = 0.0f;
+#pragma unroll 1
+  for (int k = kt0 * I4_KT; k < end; ++k) {
+    const float x = (float)a[k];
+    if (fabsf(x) < INFINITY) continue;
+    const uint32_t w = words[(size_t)(k >> 7) * 256 + (n >> 3 & 1) * 128 + ((n & 7) * 4 + (k >> 3 & 3)) * 4 + (k >> 5 & 3)];
+    v += x * (((float)(w >> 4 * (k & 7) & 15) - 8.0f) * (float)scales[(size_t)(k / group) * 16]);
+  }
+  return v;
+}
+
 // Lays out tiles [kt0, kt0 + tiles) of `rows` rows of A: 16 lanes per row and
 // tile, eight inputs each, in the order 0 4 1 5 2 6 3 7.
 template <typename T, int NT, int GB>
-__device__ __forceinline__ void i4_stage(const I4Params& p, unsigned char* xs, float* xscale, float* addend, int row0,
-                                         int rows, int kt0, int tiles) {
+__device__ __forceinline__ void i4_stage(const I4Params& p, unsigned char* xs, float* xscale, float* addend, int* special,
+                                         int row0, int rows, int kt0, int tiles) {
   constexpr int PARTS = sizeof(T) == 2 ? 1 : 2;
   constexpr int SPT = 4 / GB;
   constexpr int AHEAD = NT == 1 ? (PARTS == 1 ? 4 : 2) : 4;  // loads in flight per lane: the rows come from L2 or beyond
@@ -176,7 +196,17 @@ __device__ __forceinline__ void i4_stage(const I4Params& p, unsigned char* xs, f
         if (r >= rows) break;
         uint4 col[PARTS];
         if constexpr (PARTS == 1) {
-          const uint4 v = raw[u][0];
+          uint4 v = raw[u][0];
+          auto over = [](uint32_t w) { return (w & 0x7fff7fffu) + 0x04000400u; };  // bit 15 of a half: its exponent is all ones
+          if (((over(v.x) | over(v.y) | over(v.z) | over(v.w)) & 0x80008000u) != 0) {
+            special[r] = 1;
+            uint32_t* w = &v.x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t o = over(w[i]);
+              w[i] &= (o & 0x8000u ? 0u : 0xffffu) | (o & 0x80000000u ? 0u : 0xffff0000u);
+            }
+          }
           col[0] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
                               __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
         } else {
@@ -186,6 +216,15 @@ __device__ __forceinline__ void i4_stage(const I4Params& p, unsigned char* xs, f
           uint32_t top = 0;
 #pragma unroll
           for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+          if (top >= 0x7f800000u) {
+            special[r] = 1;
+            top = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if ((__float_as_uint(v[i]) & 0x7fffffffu) >= 0x7f800000u) v[i] = 0.0f;
+              top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+            }
+          }
 #pragma unroll
           for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
           // 2^s with the largest magnitude in [2^14, 2^15); s <= 126 keeps 2^s and 2^-s normal.
@@ -196,9 +235,7 @@ __device__ __forceinline__ void i4_stage(const I4Params& p, unsigned char* xs, f
           for (int i = 0; i < 8; ++i) {
             const float y = v[i] * up;
             hi[i] = __float2half_rn(y);
-            const float h = __half2float(hi[i]);
-            // An infinite or NaN input stands in the first column alone.
-            lo[i] = __float2half_rn(fabsf(h) <= 65504.0f ? y - h : 0.0f);
+            lo[i] = __float2half_rn(y - __half2float(hi[i]));
           }
           const int at[8] = {0, 4, 1, 5, 2, 6, 3, 7};
           __half* ha = reinterpret_cast<__half*>(&col[0]);
@@ -220,10 +257,8 @@ __device__ __forceinline__ void i4_stage(const I4Params& p, unsigned char* xs, f
           for (int o = 1; o < 4 * GB; o <<= 1) sum += __shfl_xor_sync(mask, sum, o);
           if (lane16 % (4 * GB) == 0) {
             float* dst = i4_addend<NT>(addend, kt * SPT + lane16 / (4 * GB), r * PARTS + q);
-            // An infinite sum would meet the products' infinities as a NaN; they need no addend.
-            const float v = fabsf(sum) <= 3.0e38f || sum != sum ? -72.0f * sum : 0.0f;
-            dst[0] = v;
-            dst[2] = v;
+            dst[0] = -72.0f * sum;
+            dst[2] = -72.0f * sum;
           }
         }
       }
@@ -257,6 +292,7 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
   const int stride = i4_col_bytes(p.ktiles_cta);
   float* addend = reinterpret_cast<float*>(i4_smem + (size_t)cols * stride);
   float* xscale = addend + (size_t)p.ktiles_cta * SPT * NT * 16;
+  int* special = reinterpret_cast<int*>(i4_smem + p.part_offset - I4_COLS * 4);  // rows with infinite or NaN inputs
 
   struct Slot {
     uint4 code[MT][2];
@@ -306,10 +342,12 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
   };
   // The weights too may be the previous kernel's work (a pack, a load): nothing
   // is read before it is done.
+  if (tid < I4_COLS) special[tid] = 0;
+  __syncthreads();
   pdl_entry();
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) load(ring[d]);
-  i4_stage<T, NT, GB>(p, xs, xscale, addend, row0, rows, k0, ktiles);
+  i4_stage<T, NT, GB>(p, xs, xscale, addend, special, row0, rows, k0, ktiles);
   __syncthreads();
 
   uint32_t xcol[NT], xsc[NT];  // shared memory addresses
@@ -414,6 +452,7 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
         v += src[0];
         if constexpr (PARTS == 2) v += src[M + 4];
       }
+      if (special[r] && m0 * MT * 16 + pm < p.columns) v += i4_special<T>(p, row0 + r, m0 * MT * 16 + pm, k0, ktiles);
       if (p.cluster == 1) finish(r, m0 * MT * 16 + pm, v);
       else sums[(size_t)(parity * rows + r) * M + pm] = v;
     }
@@ -530,7 +569,7 @@ int launch_typed(const DeviceCtx& dev, I4Params p, int group, cudaStream_t strea
       p.wk = std::max(1, std::min(p.ktiles_cta, warps / p.wm));
       const int spt = group == 32 ? 4 : group == 64 ? 2 : 1;
       p.part_offset = cols * i4_col_bytes(p.ktiles_cta) + p.ktiles_cta * spt * nt * 64;
-      p.part_offset = (p.part_offset + (PARTS == 2 ? p.rows_per_pass * p.ktiles_cta * 4 : 0) + 127) / 128 * 128;
+      p.part_offset = (p.part_offset + (PARTS == 2 ? p.rows_per_pass * p.ktiles_cta * 4 : 0) + I4_COLS * 4 + 127) / 128 * 128;
       smem = p.part_offset + p.wk * nt * 8 * (p.wm * mt * 16 + 4) * 4 +
              (p.cluster > 1 ? 2 * p.rows_per_pass * p.wm * mt * 16 * 4 : 0);
       if (smem <= I4_SMEM) break;

@@ -477,6 +477,43 @@ def test_int4_gemv_infinities_and_nan_stay_in_their_rows(pk, device, profile):
     assert np.all(np.isposinf(got[1])) and np.all(np.isnan(got[2])) and np.all(np.isfinite(got[[0, 3]]))
 
 
+@pytest.mark.parametrize("profile", ["fp16", "fp32"])
+@pytest.mark.parametrize("rows,inner,columns,group", [(3, 256, 40, 64), (9, 1024, 17, 128), (20, 96, 33, 32), (2, 8192, 16, 256)])
+def test_int4_gemv_infinities_take_the_weights_signs(pk, device, profile, rows, inner, columns, group):
+    """An infinity of every place of a word meets weights of both signs and zeros: the formula's signs and NaNs,
+    and the rows beside them keep the values that they have alone."""
+    import torch
+
+    rng = np.random.default_rng(31 + inner)
+    npd = np.float16 if profile == "fp16" else np.float32
+    codes = rng.integers(0, 16, (inner, columns)).astype(np.uint8)
+    scales = ((0.5 + rng.random((inner // group, columns))) * 0.05).astype(npd)
+    weight = pk.kernels.Int4Weight.from_words(torch.from_numpy(pk.runtime_plan.pack_int4(codes).view(np.int32)).cuda(),
+                                              torch.from_numpy(scales).cuda(), inner, group)
+    kernel = pk.kernels.Int4GemvKernel.create(device, None, 0, profile)
+
+    def run(a):
+        out = torch.zeros((rows, columns), dtype=_dtype(profile), device="cuda")
+        kernel.create_dispatch(dict(label="g", a=torch.from_numpy(a).cuda(), weight=weight, output=out, rows=rows)).encode()
+        return _np(out)
+
+    a = rng.standard_normal((rows, inner)).astype(npd)
+    plain = run(a)
+    w = codes.astype(np.float64) - 8.0
+    for place in range(8):
+        b = a.copy()
+        k = int(rng.integers(0, inner // 8)) * 8 + place
+        b[1, k] = -np.inf if place % 3 == 0 else np.inf
+        if place == 5:
+            b[1, (k + 8) % inner] = np.nan
+        got = run(b)
+        with np.errstate(invalid="ignore"):
+            want = np.full(columns, np.nan) if place == 5 else float(b[1, k]) * w[k]
+        np.testing.assert_array_equal(got[1], want)
+        keep = np.arange(rows) != 1
+        np.testing.assert_array_equal(got[keep], plain[keep])
+
+
 def test_int4_quantized_weight(pk, device):
     """Int4Weight.quantize end to end: the product is that of the rounded weight."""
     import torch

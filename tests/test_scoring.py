@@ -106,6 +106,54 @@ def test_joint_logits_refuses(pk, change, status, match):
     _refuse(pk, "pk_joint_logits", _joint(pk, **change), status, match)
 
 
+SCORES = ("logits", "targets", "row_count", "row_map", "log_probs", "log_sums", "entropies", "top_ids", "top_log_probs")
+GEMV = ("a", "codes", "scales", "residual", "c")
+JOINT = ("encoder_projected", "predictor", "joint_frames", "counts", "weight", "bias", "logits", "row_map", "row_count")
+NORM = ("input", "block", "post_gamma", "post_beta", "pre_gamma", "gate", "output", "normalized")
+
+
+@pytest.mark.parametrize("entry,make,names,a,b,shift", [
+    ("pk_token_scores", _scores, SCORES, "log_probs", "logits", 4),
+    ("pk_token_scores", _scores, SCORES, "log_probs", "targets", 0),
+    ("pk_token_scores", _scores, SCORES, "top_ids", "top_log_probs", 8),
+    ("pk_token_scores", _scores, SCORES, "entropies", "row_map", 8),
+    ("pk_token_scores", _scores, SCORES, "log_sums", "row_count", -8),
+    ("pk_int4_gemv", _gemv, GEMV, "c", "a", 0),
+    ("pk_int4_gemv", _gemv, GEMV, "c", "residual", 2),
+    ("pk_int4_gemv", _gemv, GEMV, "c", "codes", 1024),
+    ("pk_int4_gemv", _gemv, GEMV, "c", "scales", 0),
+    ("pk_joint_logits", _joint, JOINT, "logits", "encoder_projected", 512),
+    ("pk_joint_logits", _joint, JOINT, "logits", "predictor", 16),
+    ("pk_joint_logits", _joint, JOINT, "row_map", "joint_frames", 0),
+    ("pk_joint_logits", _joint, JOINT, "row_count", "counts", 4),
+    ("pk_joint_logits", _joint, JOINT, "row_map", "row_count", -4),
+    ("pk_residual_norm", _norm, NORM, "output", "pre_gamma", 0),
+    ("pk_residual_norm", _norm, NORM, "normalized", "gate", 128),
+])
+def test_outputs_over_other_buffers_are_refused(pk, entry, make, names, a, b, shift):
+    at = {n: (100 + i) * P for i, n in enumerate(names)}
+    at[a] = at[b] + shift
+    _refuse(pk, entry, make(pk, **at), -1, "overlap")
+
+
+@pytest.mark.parametrize("entry,make,names,name,by", [
+    ("pk_token_scores", _scores, SCORES, "targets", 2), ("pk_token_scores", _scores, SCORES, "top_ids", 1),
+    ("pk_token_scores", _scores, SCORES, "row_map", 2), ("pk_int4_gemv", _gemv, GEMV, "c", 1),
+    ("pk_int4_gemv", _gemv, GEMV, "scales", 1), ("pk_int4_gemv", _gemv, GEMV, "residual", 1),
+    ("pk_joint_logits", _joint, JOINT, "counts", 2), ("pk_joint_logits", _joint, JOINT, "row_count", 2),
+    ("pk_joint_logits", _joint, JOINT, "logits", 8), ("pk_residual_norm", _norm, NORM, "gate", 2),
+])
+def test_buffers_off_their_elements_are_refused(pk, entry, make, names, name, by):
+    at = {n: (100 + i) * P for i, n in enumerate(names)}
+    at[name] += by
+    _refuse(pk, entry, make(pk, **at), -3, "aligned")
+
+
+def test_token_scores_refuses_sizes_that_no_memory_holds(pk):
+    for change in (dict(row_stride=1 << 60), dict(slots=(1 << 32) + 1)):
+        _refuse(pk, "pk_token_scores", _scores(pk, **change), -2, "at most")
+
+
 # ------------------------------------------------------------------ dispatches
 
 def test_dispatches_refuse_shapes_before_buffers(pk):
@@ -228,6 +276,9 @@ def test_trace_and_alternatives_are_refused(pk):
     for tr in (None, ctypes.byref(trace)):
         with pytest.raises(pk.PkError, match="trace"):
             lib.call("pk_tdt_decode_traced", ctypes.cast(buf, ctypes.c_void_p), ctypes.byref(desc), tr, None)
+    for shifted in (lib.TdtTrace(P + 8, P), lib.TdtTrace(P, P + 2)):
+        with pytest.raises(pk.PkError, match="aligned"):
+            lib.call("pk_tdt_decode_traced", ctypes.cast(buf, ctypes.c_void_p), ctypes.byref(desc), ctypes.byref(shifted), None)
     for k in (-1, 33):
         with pytest.raises(pk.kernels.RangeError, match="alternatives"):
             pk.engine.ParakeetEngine(_FakeDevice(), {}, "fp16", alternatives=k)
