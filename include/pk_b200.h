@@ -307,9 +307,9 @@ int pk_residual_norm(pk_device* device, const pk_residual_norm_desc* desc, pk_st
  * The scale multiplies the group's f32 sum; an infinite or NaN input adds its
  * product as the formula does.  Epilogue as in pk_gemm_desc; bias
  * and residual are exclusive.  Codes lie in tiles of 16 outputs x 128 inputs
- * ("n16-k128-lane-major-int4-u32"): u32 [ceil(N / 16)][ceil(K / 128)][2][32][4],
- * where word i of lane l in half h holds, lowest bits first, the codes of
- * inputs 128 kt + 32 i + 8 (l % 4) + 0..7 of output 16 nt + 8 h + l / 4; places
+ * ("n16-k128-tile-int4-u32"): u32 [ceil(N / 16)][ceil(K / 128)][16][4][4],
+ * where word [o][(t + o / 2) % 4][i] of a tile holds, lowest bits first, the
+ * codes of inputs 128 kt + 32 i + 8 t + 0..7 of output 16 nt + o; places
  * outside the matrix hold code 8.  Scales lie as
  * [ceil(N / 16)][K / group][16] ("n16-k-group-major-scale"), zero outside. */
 typedef struct pk_int4_gemv_desc {
@@ -324,7 +324,7 @@ typedef struct pk_int4_gemv_desc {
   const void* residual;      /* device [rows, N] or NULL: C = residual + residual_scale * value; may be C */
   const void* a;             /* device [rows, K], 16-byte aligned */
   const uint32_t* codes;     /* device, 16-byte aligned */
-  const void* scales;        /* device [ceil(N / 16), K / group, 16] */
+  const void* scales;        /* device [ceil(N / 16), K / group, 16], 16-byte aligned */
   void* c;                   /* device [rows, N] */
 } pk_int4_gemv_desc;
 int pk_int4_gemv(pk_device* device, const pk_int4_gemv_desc* desc, pk_stream stream);

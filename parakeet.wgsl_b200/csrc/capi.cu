@@ -509,7 +509,7 @@ int pk_int4_gemv(pk_device* device, const pk_int4_gemv_desc* d, pk_stream stream
   const int st = check_spans("int4 product", {c},
                              {{"a", d->a, d->rows * d->inner * es, 16},
                               {"codes", d->codes, tiles * ((d->inner + 127) / 128) * 1024, 16},
-                              {"scales", d->scales, tiles * (d->inner / d->group) * 16 * es, es},
+                              {"scales", d->scales, tiles * (d->inner / d->group) * 16 * es, 16},
                               {"bias", d->bias, 4 * d->columns, 4},
                               residual});
   if (st != PK_OK) return st;

@@ -5,16 +5,18 @@
 //
 // Bound by reading the codes once (half a byte a weight), so what matters is
 // that the codes stream without a pause and that a weight costs few
-// instructions.  The product runs on mma.sync m16n8k16 with the weights as the
-// 16-row operand and the rows of A as the 8 columns: tcgen05 would have to
-// take the weights through shared memory first, and its 128-row tiles would
-// stay empty for the sake of a rate that this operator cannot use.
+// instructions.  Here, for up to 16 columns and for small matrices, the product
+// runs on mma.sync m16n8k16 with the weights as the 16-row operand and the rows
+// of A as the 8 columns: its operand is expanded in the registers that it is
+// loaded to, a warp needs no other, and no tile is larger than the work.
+// int4_umma.cu has the rest.
 //
-// Codes lie in tiles of 16 outputs x 128 inputs (1 KB) in the order in which a
-// warp's lanes hold the matrix operand, so a lane reads two 16-byte words per
-// tile and a warp 512 contiguous bytes at a time, four tiles ahead.  Word i of
-// a lane holds inputs 32 i + 8 t .. + 7 (t = lane % 4) of outputs lane / 4 (+ 8
-// in the second 16 bytes).  A code becomes f16 by placing its 4 bits in a
+// Codes lie in tiles of 16 outputs x 128 inputs (1 KB), 64 bytes an output, so a
+// lane reads two 16-byte words per tile and a warp 512 contiguous bytes at a
+// time.  Word i of a lane holds inputs 32 i + 8 t .. + 7 (t = lane % 4) of
+// outputs lane / 4 (+ 8 in the second 16 bytes); the four t of an output are
+// turned by output / 2, so that a thread per output reads them from shared
+// memory without bank conflicts too.  A code becomes f16 by placing its 4 bits in a
 // mantissa: 1024 + code where they are the lowest, less 1032 in one more
 // instruction; 64 + code where they are the next four, which stays as it is --
 // the sums of a group begin at -72 times the sum of those inputs instead (the
@@ -42,16 +44,12 @@
 #include <mutex>
 #include <utility>
 
-#include "pk_common.cuh"
-#include "pk_internal.h"
+#include "int4_common.cuh"
 
 namespace pk {
 namespace {
 
-constexpr int I4_KT = 128;        // inputs per tile
 constexpr int I4_COLS = 32;       // columns of one pass, at most (more rows: the codes again, from L2)
-constexpr int I4_CLUSTER = 8;     // CTAs that share the inputs, at most
-constexpr int I4_SMEM = 220 * 1024;
 
 // Warps per CTA (registers: 72, 128, 128 a thread), tiles of outputs a warp takes
 // at a time and tiles in flight per warp, by column tiles.  With two output
@@ -60,33 +58,6 @@ constexpr int I4_SMEM = 220 * 1024;
 __host__ __device__ constexpr int i4_warps(int nt) { return nt == 1 ? 28 : 16; }
 __host__ __device__ constexpr int i4_mt(int nt) { return nt == 2 ? 2 : 1; }
 __host__ __device__ constexpr int i4_depth(int nt) { return nt == 2 ? 2 : 3; }
-
-struct I4Params {
-  const void* a;
-  const uint4* codes;
-  const void* scales;
-  const float* bias;
-  const void* residual;
-  void* c;
-  int rows, inner, columns, ktiles;
-  int groups;           // scales per output
-  uint32_t group_inv;   // 2^32 / (tiles per group), rounded up (groups of whole tiles)
-  int wm, wk;           // warps over outputs, over inputs
-  int ktiles_cta;       // tiles of inputs per CTA of a cluster
-  int cluster;
-  int rows_per_pass;
-  int part_offset;      // bytes of shared memory before the parts
-  int act;
-  float residual_scale;
-};
-
-__device__ __forceinline__ uint32_t i4_lop(uint32_t a, uint32_t b, uint32_t c) {  // (a & b) | c
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-__device__ __forceinline__ uint32_t i4_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 i4_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
 // Eight codes -> the pairs (0,4) (2,6) of code - 8 and (1,5) (3,7) of code + 64.
 __device__ __forceinline__ void i4_expand(uint32_t w, uint32_t (&p)[4]) {
@@ -113,25 +84,6 @@ __device__ __forceinline__ void i4_mma_first(float (&d)[4], uint32_t a0, uint32_
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(__uint_as_float(c.x)), "f"(__uint_as_float(c.y)), "f"(__uint_as_float(c.z)), "f"(__uint_as_float(c.w)));
 }
 
-__device__ __forceinline__ uint4 i4_load(const uint4* p) {
-  uint4 v;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-      : "l"(p));
-  return v;
-}
-
-__device__ __forceinline__ uint4 i4_lds(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ float i4_lds_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
-  return v;
-}
-
 // Bytes of one column of staged inputs: the columns of a quarter warp's loads
 // fall on different banks.
 __host__ __device__ inline int i4_col_bytes(int ktiles) { return ktiles * I4_KT * 2 + 64; }
@@ -142,25 +94,6 @@ __host__ __device__ inline int i4_col_bytes(int ktiles) { return ktiles * I4_KT 
 template <int NT>
 __device__ __forceinline__ float* i4_addend(float* base, int block, int col) {
   return base + (size_t)(block * NT * 4 + (col >> 1)) * 4 + (col & 1);
-}
-
-// The products of row r's infinite and NaN inputs of tiles [kt0, kt0 + tiles) with output n.
-template <typename T>
-__device__ float i4_special(const I4Params& p, int r, int n, int kt0, int tiles) {
-  const T* a = static_cast<const T*>(p.a) + (size_t)r * p.inner;
-  const uint32_t* words = reinterpret_cast<const uint32_t*>(p.codes) + ((size_t)(n >> 4) * p.ktiles) * 256;
-  const T* scales = static_cast<const T*>(p.scales) + (size_t)(n >> 4) * p.groups * 16 + (n & 15);
-  const int group = p.inner / p.groups;
-  const int end = min((kt0 + tiles) * I4_KT, p.inner);
-  float v = 0.0f;
-#pragma unroll 1
-  for (int k = kt0 * I4_KT; k < end; ++k) {
-    const float x = (float)a[k];
-    if (fabsf(x) < INFINITY) continue;
-    const uint32_t w = words[(size_t)(k >> 7) * 256 + (n >> 3 & 1) * 128 + ((n & 7) * 4 + (k >> 3 & 3)) * 4 + (k >> 5 & 3)];
-    v += x * (((float)(w >> 4 * (k & 7) & 15) - 8.0f) * (float)scales[(size_t)(k / group) * 16]);
-  }
-  return v;
 }
 
 // Lays out tiles [kt0, kt0 + tiles) of `rows` rows of A: 16 lanes per row and
@@ -195,58 +128,9 @@ __device__ __forceinline__ void i4_stage(const I4Params& p, unsigned char* xs, f
         const int r = r0 + u * side;
         if (r >= rows) break;
         uint4 col[PARTS];
-        if constexpr (PARTS == 1) {
-          uint4 v = raw[u][0];
-          auto over = [](uint32_t w) { return (w & 0x7fff7fffu) + 0x04000400u; };  // bit 15 of a half: its exponent is all ones
-          if (((over(v.x) | over(v.y) | over(v.z) | over(v.w)) & 0x80008000u) != 0) {
-            special[r] = 1;
-            uint32_t* w = &v.x;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t o = over(w[i]);
-              w[i] &= (o & 0x8000u ? 0u : 0xffffu) | (o & 0x80000000u ? 0u : 0xffff0000u);
-            }
-          }
-          col[0] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
-                              __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-        } else {
-          float v[8];
-          *reinterpret_cast<uint4*>(v) = raw[u][0];
-          *reinterpret_cast<uint4*>(v + 4) = raw[u][PARTS - 1];
-          uint32_t top = 0;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-          if (top >= 0x7f800000u) {
-            special[r] = 1;
-            top = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if ((__float_as_uint(v[i]) & 0x7fffffffu) >= 0x7f800000u) v[i] = 0.0f;
-              top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-            }
-          }
-#pragma unroll
-          for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
-          // 2^s with the largest magnitude in [2^14, 2^15); s <= 126 keeps 2^s and 2^-s normal.
-          const int s = min(141 - (int)(top >> 23), 126);
-          const float up = __uint_as_float((uint32_t)(s + 127) << 23), down = __uint_as_float((uint32_t)(127 - s) << 23);
-          __half hi[8], lo[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float y = v[i] * up;
-            hi[i] = __float2half_rn(y);
-            lo[i] = __float2half_rn(y - __half2float(hi[i]));
-          }
-          const int at[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-          __half* ha = reinterpret_cast<__half*>(&col[0]);
-          __half* hb = reinterpret_cast<__half*>(&col[PARTS - 1]);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            ha[i] = hi[at[i]];
-            hb[i] = lo[at[i]];
-          }
-          if (lane16 == 0) xscale[r * p.ktiles_cta + kt] = down;
-        }
+        float down = 1.0f;
+        if (i4_columns<T>(raw[u], mask, col, down)) special[r] = 1;
+        if (PARTS == 2 && lane16 == 0) xscale[r * p.ktiles_cta + kt] = down;
 #pragma unroll
         for (int q = 0; q < PARTS; ++q) {
           *reinterpret_cast<uint4*>(xs + (size_t)(r * PARTS + q) * stride + kt * (I4_KT * 2) + lane16 * 16) = col[q];
@@ -312,7 +196,7 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int mt = min(lm * MT + m, mtiles - 1);
-      lcode[m] = p.codes + ((size_t)mt * p.ktiles + k0 + lk) * 64 + lane;
+      lcode[m] = p.codes + ((size_t)mt * p.ktiles + k0 + lk) * 64 + 4 * g + ((t + (g >> 1)) & 3);
       lscale[m] = static_cast<const T*>(p.scales) + (size_t)mt * p.groups * 16 + g;
     }
   };
@@ -436,14 +320,11 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
         for (int e = 0; e < 4; ++e)
           part[((size_t)wk * PC + n * 8 + 2 * t + (e & 1)) * (M + 4) + (wm * MT + m) * 16 + g + 8 * (e >> 1)] = total[m][n][e];
     __syncthreads();
-    auto finish = [&](int r, int n, float v) {
+    auto finish = [&](int r, float v) {
+      const int n = m0 * MT * 16 + pm;
       if (n >= p.columns) return;
       if (p.bias) v += __ldg(p.bias + n);
-      if (p.act == PK_ACT_SILU) v = v / (1.0f + expf(-v));
-      else if (p.act == PK_ACT_RELU) v = v < 0.0f ? 0.0f : v;
-      const size_t at = (size_t)(row0 + r) * p.columns + n;
-      if (p.residual) v = fmaf(p.residual_scale, v, (float)static_cast<const T*>(p.residual)[at]);
-      static_cast<T*>(p.c)[at] = (T)v;
+      i4_finish<T>(p, (size_t)(row0 + r) * p.columns + n, v);
     };
     for (int r = pr; r < rows; r += rstep) {
       float v = 0.0f;
@@ -453,7 +334,7 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
         if constexpr (PARTS == 2) v += src[M + 4];
       }
       if (special[r] && m0 * MT * 16 + pm < p.columns) v += i4_special<T>(p, row0 + r, m0 * MT * 16 + pm, k0, ktiles);
-      if (p.cluster == 1) finish(r, m0 * MT * 16 + pm, v);
+      if (p.cluster == 1) finish(r, v);
       else sums[(size_t)(parity * rows + r) * M + pm] = v;
     }
     __syncthreads();  // the parts are read (and the sums written)
@@ -471,7 +352,7 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
 #pragma unroll
         for (int c = 0; c < I4_CLUSTER; ++c)
           if (c < p.cluster) v += u[c];
-        finish(r, m0 * MT * 16 + pm, v);
+        finish(r, v);
       }
     }
   }
@@ -479,41 +360,6 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
     __syncwarp();
     cluster_sync();  // no CTA leaves while another reads its sums
   }
-}
-
-// Clusters of `cluster` CTAs that run at once with one CTA per SM (fewer than
-// SMs / cluster: a cluster stays within a GPC, and GPCs differ in size).
-int i4_clusters(const DeviceCtx& dev, int cluster, int* out) {
-  if (cluster == 1) {
-    *out = dev.sm_count;
-    return PK_OK;
-  }
-  static std::mutex mu;
-  static std::map<std::pair<int, int>, int> known;
-  std::lock_guard<std::mutex> lock(mu);
-  int& n = known[{dev.ordinal, cluster}];
-  if (n == 0) {
-    const void* kernel = reinterpret_cast<const void*>(int4_gemv_kernel<__half, 1, 4>);
-    const int st = set_max_dynamic_smem(kernel, I4_SMEM);
-    if (st != PK_OK) return st;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)cluster;
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)cluster);
-    cfg.blockDim = dim3(i4_warps(1) * 32);
-    cfg.dynamicSmemBytes = I4_SMEM;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    int most = 0;
-    const cudaError_t e = cudaOccupancyMaxActiveClusters(&most, kernel, &cfg);
-    if (e != cudaSuccess) return cuda_error(e, "occupancy query (int4 product)");
-    n = std::max(1, most);
-  }
-  *out = n;
-  return PK_OK;
 }
 
 template <typename T, int NT, int GB>
@@ -561,7 +407,7 @@ int launch_typed(const DeviceCtx& dev, I4Params p, int group, cudaStream_t strea
       // Few outputs: the inputs over more SMs, while each has a tile for every warp of 4.
       if (mgroups * p.cluster * 2 <= dev.sm_count && p.cluster < I4_CLUSTER && p.ktiles >= p.cluster * 2 * 4) continue;
       p.ktiles_cta = (p.ktiles + p.cluster - 1) / p.cluster;
-      const int st = i4_clusters(dev, p.cluster, &clusters);
+      const int st = int4_clusters(dev, p.cluster, &clusters);
       if (st != PK_OK) return st;
       const int q = (mgroups + clusters - 1) / clusters;  // groups of outputs of a cluster
       const int turns = (q + warps - 1) / warps;
@@ -585,7 +431,51 @@ int launch_typed(const DeviceCtx& dev, I4Params p, int group, cudaStream_t strea
   return launch_group<T, 4>(p, group, grid, smem, stream);
 }
 
+// tcgen05 takes more than 16 columns, and five tiles of 128 x 128 weights per SM
+// (counted once per 32 columns).  Below that its pipeline is not filled, and its
+// tiles are too coarse to share out (32x1024x4096 f16: 8.3 us against 7.0 here);
+// above it, 32x4096x8192 f16 takes 15.0 us against 22.3, 64x4096x4096 21.5
+// against 27.1.  With 16 columns it is behind: 16x4096x65536 f16 55 us against 49.
+bool umma_route(const DeviceCtx& dev, const I4Params& p, int parts) {
+  const int64_t columns = (int64_t)p.rows * parts, tiles = (int64_t)((p.columns + 127) / 128) * p.ktiles;
+  return columns > 16 && tiles * ((columns + I4_COLS - 1) / I4_COLS) >= 5 * dev.sm_count;
+}
+
 }  // namespace
+
+// Fewer than SMs / cluster: a cluster stays within a GPC, and GPCs differ in size.
+int int4_clusters(const DeviceCtx& dev, int cluster, int* out) {
+  if (cluster == 1) {
+    *out = dev.sm_count;
+    return PK_OK;
+  }
+  static std::mutex mu;
+  static std::map<std::pair<int, int>, int> known;
+  std::lock_guard<std::mutex> lock(mu);
+  int& n = known[{dev.ordinal, cluster}];
+  if (n == 0) {
+    const void* kernel = reinterpret_cast<const void*>(int4_gemv_kernel<__half, 1, 4>);
+    const int st = set_max_dynamic_smem(kernel, I4_SMEM);
+    if (st != PK_OK) return st;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)cluster;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)cluster);
+    cfg.blockDim = dim3(i4_warps(1) * 32);
+    cfg.dynamicSmemBytes = I4_SMEM;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int most = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&most, kernel, &cfg);
+    if (e != cudaSuccess) return cuda_error(e, "occupancy query (int4 product)");
+    n = std::max(1, most);
+  }
+  *out = n;
+  return PK_OK;
+}
 
 int launch_int4_gemv(const DeviceCtx& dev, const pk_int4_gemv_desc& d, cudaStream_t stream) {
   I4Params p{};
@@ -605,6 +495,8 @@ int launch_int4_gemv(const DeviceCtx& dev, const pk_int4_gemv_desc& d, cudaStrea
   p.group_inv = per > 1 ? (uint32_t)((((uint64_t)1 << 32) + per - 1) / per) : 0u;
   p.act = d.activation;
   p.residual_scale = d.residual_scale;
+  p.status = dev.status;
+  if (umma_route(dev, p, d.precision == PK_FP16 ? 1 : 2)) return launch_int4_umma(dev, p, d.precision, (int)d.group, stream);
   return d.precision == PK_FP16 ? launch_typed<__half>(dev, p, (int)d.group, stream)
                                 : launch_typed<float>(dev, p, (int)d.group, stream);
 }

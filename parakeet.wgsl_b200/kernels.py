@@ -875,8 +875,10 @@ class Int4Weight:
             full = torch.full((nt * 16, kt * 16), -0x77777778, dtype=torch.int32, device=w.device)
             full[:columns, :inner // 8] = w
             w = full
-        # [tile row, half, lane / 4, tile column, block of 32 inputs, lane % 4]
-        tiles = w.reshape(nt, 2, 8, kt, 4, 4).permute(0, 3, 1, 2, 5, 4).contiguous().reshape(-1)
+        # [tile row, output of 16, tile column, block of 32 inputs, eight of the block], the eights turned by output / 2
+        tiles = w.reshape(nt, 16, kt, 4, 4).permute(0, 2, 1, 4, 3)
+        outputs, places = torch.arange(16, device=w.device)[:, None], torch.arange(4, device=w.device)
+        tiles = tiles[:, :, outputs, (places - outputs // 2) % 4].contiguous().reshape(-1)
         padded = torch.zeros((inner // group, nt * 16), dtype=scales.dtype, device=w.device) if columns % 16 else scales
         if columns % 16:
             padded[:, :columns] = scales

@@ -29,7 +29,7 @@ PALETTE5_LAYOUT = "k-by-output-row-major-palette5-lsb-u32"
 PALETTE6_LAYOUT = "k-by-output-row-major-palette6-lsb-u32"
 PALETTE_LUT_LAYOUT = "output-group-by-palette-lut"
 INT4_LAYOUT = "output-by-k-int4-lsb-u32"
-INT4_TILE_LAYOUT = "n16-k128-lane-major-int4-u32"
+INT4_TILE_LAYOUT = "n16-k128-tile-int4-u32"
 INT4_TILE_SCALE_LAYOUT = "n16-k-group-major-scale"
 TILE_INNER = 32
 

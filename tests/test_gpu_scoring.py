@@ -440,6 +440,17 @@ def test_int4_gemv(pk, device, profile, rows, inner, columns, group):
     _int4(pk, device, rows, inner, columns, group, profile)
 
 
+# Enough rows and tiles for the tcgen05 route: five tiles of 128 x 128 weights per SM and 32 columns.
+@pytest.mark.parametrize("profile", ["fp16", "fp32"])
+@pytest.mark.parametrize("rows,inner,columns,group,epilogue", [
+    (17, 1056, 12005, 32, "none"), (17, 640, 19000, 64, "bias"), (32, 4096, 4001, 128, "silu"), (33, 128, 97000, 128, "none"),
+    (64, 8192, 1500, 512, "residual"), (20, 32768, 300, 128, "residual in place"), (19, 2208, 6100, 32, "relu"),
+    (64, 96, 50000, 32, "none"), (23, 16384, 1000, 64, "none"),
+])
+def test_int4_gemv_many_rows(pk, device, profile, rows, inner, columns, group, epilogue):
+    _int4(pk, device, rows, inner, columns, group, profile, epilogue)
+
+
 @pytest.mark.parametrize("profile", ["fp16", "fp32"])
 @pytest.mark.parametrize("epilogue", ["bias", "silu", "relu", "residual", "residual in place"])
 @pytest.mark.parametrize("rows", [1, 12])
@@ -478,7 +489,7 @@ def test_int4_gemv_infinities_and_nan_stay_in_their_rows(pk, device, profile):
 
 
 @pytest.mark.parametrize("profile", ["fp16", "fp32"])
-@pytest.mark.parametrize("rows,inner,columns,group", [(3, 256, 40, 64), (9, 1024, 17, 128), (20, 96, 33, 32), (2, 8192, 16, 256)])
+@pytest.mark.parametrize("rows,inner,columns,group", [(3, 256, 40, 64), (9, 1024, 17, 128), (20, 96, 33, 32), (2, 8192, 16, 256), (20, 2048, 6000, 128)])
 def test_int4_gemv_infinities_take_the_weights_signs(pk, device, profile, rows, inner, columns, group):
     """An infinity of every place of a word meets weights of both signs and zeros: the formula's signs and NaNs,
     and the rows beside them keep the values that they have alone."""

@@ -181,3 +181,37 @@ def test_scores_repeat_while_their_graph_replays_elsewhere(pk, device):
     torch.cuda.synchronize()
     for _, _, outs, host in progs:
         t._check_chain(pk, outs, host, "fp32")
+
+
+def test_int4_gemv_repeats_bit_for_bit_on_streams_and_in_graphs(pk, device):
+    """The tcgen05 route (32 columns, 32 tiles per SM) on two streams at once and replayed: always the same bits."""
+    import torch
+
+    rng = np.random.default_rng(51)
+    inner, columns, group = 4096, 16384, 128
+    K = pk.kernels
+    weight = K.Int4Weight.quantize((rng.standard_normal((inner, columns)) * 0.02).astype(np.float32), group, "fp16")
+    a = torch.randn((32, inner), device="cuda").half()
+    outs = [torch.zeros((32, columns), dtype=torch.float16, device="cuda") for _ in range(3)]
+    calls = [K.Int4GemvKernel.create(device).create_dispatch(dict(label="g", a=a, weight=weight, output=o, rows=32)) for o in outs]
+    calls[0].encode()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for c, s in zip(calls[1:], streams):
+            c.encode(s)
+    torch.cuda.synchronize()
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls[1].encode()
+        calls[2].encode()
+    for o in outs[1:]:
+        o.zero_()
+    for _ in range(5):
+        graph.replay()
+    torch.cuda.synchronize()
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
+    device.status()
