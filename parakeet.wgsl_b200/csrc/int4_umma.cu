@@ -80,13 +80,6 @@ __device__ __forceinline__ void iu_cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// One lane of the warp.
-__device__ __forceinline__ bool iu_elect() {
-  uint32_t one;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(one));
-  return one != 0;
-}
-
 // D (+)= A B with A in TMEM: lane = row, 16 f16 in eight columns.
 __device__ __forceinline__ void iu_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -227,7 +220,7 @@ __global__ void __launch_bounds__(IU_THREADS, 1) int4_umma_kernel(const I4Params
   const int quad = warp & 3, row = quad * 32 + lane;  // the TMEM lane: an output of the tile
   // The loads of tile `c` into stage s: eight tiles of 16 outputs.  One lane
   // issues them (lanes in turn took 120 cycles a copy, one takes 30).
-  const bool leader = iu_elect();
+  const bool leader = elect_one();
   const int last_m16 = (p.columns + 15) / 16 - 1;  // outputs behind it are not stored
   auto load = [&](const Cursor& c, uint32_t s) {
     if (leader) {

@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(jl_rows<T>() + 64, 1) joint_logits_kernel(cons
   uint32_t used = 0;
   if (warp == ROWS / 32) {
     // ------------------------------------------------------------ MMAs
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t idesc = (F16 ? umma_idesc_f16(JL_M, 0, 0, /*weight, MN-major*/ 1) : umma_idesc_tf32(JL_M, 0)) |
                              ((uint32_t)(bn >> 3) << 17);
       uint32_t turn = 0;
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(jl_rows<T>() + 64, 1) joint_logits_kernel(cons
     }
   } else if (warp == ROWS / 32 + 1) {
     // ------------------------------------------------------------ weights
-    if (lane == 0) {
+    if (elect_one()) {
       const int boxes = F16 ? (bn + 63) / 64 : 1;
       uint64_t* read = F16 ? empty : unpacked;
       bool good = true;
