@@ -15,8 +15,8 @@
 // still rank (NaN as -inf).  A row of -inf alone scores -inf with entropy 0.
 //
 // Two routes.  HELD: the warps of a row hold it in registers, so the maximum
-// is known before the first exponential.  STREAM: longer rows pass through
-// once with a running (m, s, u) per thread.
+// is known before the first exponential; for few rows.  STREAM: many or long
+// rows pass through once with a running (m, s, u) per thread.
 //
 // Alternatives cost nothing while the row is read: a lane knows its largest
 // value, and the K-th largest of any maxima of parts of the row bounds the K-th
@@ -46,6 +46,7 @@ constexpr int TS_CLUSTER = 8;            // CTAs that share a row, at most
 constexpr int TS_HELD = 10;              // 16-byte vectors per lane of a held row, at most
 constexpr int TS_HELD_FEW = 4;           // and where there are few rows: more warps, shorter chains
 constexpr int TS_AGAIN = 2;              // lanes whose vectors are read again at a time
+constexpr int64_t TS_LIVE = 114000000;   // bytes of rows under way, at most: most of L2
 constexpr int TS_UNR = 4;                // vectors per lane and tile of a streamed row
 constexpr int TS_POOL = 128;             // candidates per warp of a row
 constexpr uint32_t TS_MASKED = 0x007fffffu;  // ts_ordered(-inf)
@@ -641,21 +642,32 @@ int launch_typed(const DeviceCtx& dev, const TsParams& p, cudaStream_t stream) {
     while (w * 32 * nv < vectors) w *= 2;
     return w;
   };
-  // Few rows: every warp holds little, over as many SMs as there are.
-  int64_t few = warps_for(TS_HELD_FEW);
-  if (p.k > 16) few = std::max<int64_t>(few, 2);
+  // More alternatives than half a warp's lanes: one warp's 32 lane maxima would bound them too loosely.
+  const int64_t least = p.k > 16 ? 2 : 1;
+  // Few rows: every warp holds little, over as many SMs as there are (1x32000 f16
+  // 6.3 us against 7.1 with TS_HELD vectors a lane and 8.6 streamed; 1x131072 9.1,
+  // 14.7 without a cluster).
+  const int64_t few = std::max(warps_for(TS_HELD_FEW), least);
   if (few <= TS_WARPS * TS_CLUSTER && p.rows * few <= (int64_t)dev.sm_count * TS_WARPS)
     return launch_route<T, TS_HELD_FEW>(p, (int)std::min<int64_t>(few, TS_WARPS), (int)std::max<int64_t>(1, few / TS_WARPS),
                                         stream);
-  int64_t held = warps_for(TS_HELD);
-  // More alternatives than half a warp's lanes: 32 lane maxima would bound them too loosely.
-  if (p.k > 16) held = std::max<int64_t>(held, 2);
-  if (held <= TS_WARPS) return launch_route<T, TS_HELD>(p, (int)held, 1, stream);
+  // Rows that all run at once (two CTAs an SM): held, one round trip to memory
+  // (1000x4096 f16 8.4 us against 12.5 streamed, 1953x1025 f32 6.4 against 10.0).
+  // More rows are streamed, by warps that come and go with more of them on an SM
+  // (16384x4096 f16 51 us against 99 held, 4096x8192 23 against 53).
+  const int64_t held = std::max(warps_for(TS_HELD), least);
+  if (held <= TS_WARPS && p.rows * held <= 2 * (int64_t)dev.sm_count * TS_WARPS) return launch_route<T, TS_HELD>(p, (int)held, 1, stream);
   if (held <= TS_WARPS * TS_CLUSTER && p.rows * held <= (int64_t)dev.sm_count * TS_WARPS)
     return launch_route<T, TS_HELD>(p, TS_WARPS, (int)(held / TS_WARPS), stream);
+  // Streamed: a warp per row costs least (4096x8192 f16 23 us, 30 with two, 42 with
+  // four, 48 with eight), as long as the rows fill the SMs and those under way
+  // stay in L2, from where candidates are read again (4096x50257: 133, 129, 115, 105).
   int cluster = 1;
   while (cluster < TS_CLUSTER && p.rows * cluster * 2 <= dev.sm_count) cluster *= 2;
-  return launch_route<T, 0>(p, TS_WARPS, cluster, stream);
+  const int64_t warps = (int64_t)dev.sm_count * 4 * TS_WARPS;  // at once
+  int wpr = cluster > 1 ? TS_WARPS : (int)least;
+  while (wpr < TS_WARPS && (p.rows * wpr * 2 <= warps || warps / wpr * p.columns * (int64_t)sizeof(T) > TS_LIVE)) wpr *= 2;
+  return launch_route<T, 0>(p, wpr, cluster, stream);
 }
 
 }  // namespace

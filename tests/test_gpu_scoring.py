@@ -170,6 +170,42 @@ def test_token_scores_of_rows_without_a_distribution(pk, device, columns):
     assert np.all(np.isnan(got["log_probs"][3:])) and np.all(np.isfinite(got["log_sums"][3:]))
 
 
+@pytest.mark.parametrize("profile", ["fp16", "fp32"])
+@pytest.mark.parametrize("rows,columns,stride,first,k", [
+    (4801, 1, 1, 0, 1), (4801, 100, 101, 0, 5), (2600, 1025, 1032, 0, 32), (4800, 1025, 1033, 3, 17), (2500, 2100, 2100, 0, 0),
+    (5000, 4099, 4104, 5, 8), (2400, 9000, 9000, 0, 20), (1300, 21000, 21001, 1, 6),
+])
+def test_token_scores_of_many_rows(pk, device, profile, rows, columns, stride, first, k):
+    """Rows by the thousand: one or more warps to a row, streamed."""
+    test_token_scores(pk, device, profile, rows, columns, stride, first, k)
+
+
+@pytest.mark.parametrize("profile", ["fp16", "fp32"])
+def test_token_scores_of_many_rows_with_masks_and_ties(pk, device, profile):
+    """Masked columns, rows of equal values (whose candidates overflow the pool) and rows without a distribution
+    give the same among thousands of rows as in a call of their own."""
+    import torch
+
+    rng = np.random.default_rng(61)
+    x = _logits(rng, 4800, 3001, profile)
+    x[7], x[1200] = -np.inf, x.dtype.type(1.5)
+    x[2400, 1:] = -np.inf
+    x[3000, ::3] = x[3000, 0]
+    x[4000, 17], x[4799, 5] = np.nan, np.inf
+    targets = rng.integers(0, 3001, 4800).astype(np.int32)
+    names = ("log_probs", "log_sums", "entropies", "top_ids", "top_log_probs")
+    for k in (4, 24):
+        many = Scores(pk, device, torch.from_numpy(x).cuda(), 3001, profile, torch.from_numpy(targets).cuda(), k)().host()
+        at = np.array([7, 1200, 2400, 3000, 4000, 4799, 11])
+        few = Scores(pk, device, torch.from_numpy(np.ascontiguousarray(x[at])).cuda(), 3001, profile,
+                     torch.from_numpy(targets[at]).cuda(), k)().host()
+        for n in names:
+            if n == "top_ids":
+                np.testing.assert_array_equal(many[n][at], few[n])
+            else:  # two orders of the same f32 sums of 3001 terms: 2 * (3001 / 32 + 40) roundings at most, log sum below 13
+                np.testing.assert_allclose(many[n][at], few[n], rtol=0, atol=2 * (3001 / 32 + 40) * E * 13, equal_nan=True)
+
+
 def test_token_scores_row_count_and_row_map(pk, device):
     """Rows behind the device's count, slots outside the buffers and slots nobody maps to stay as they were."""
     import torch
