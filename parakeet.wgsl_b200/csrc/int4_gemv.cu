@@ -32,6 +32,11 @@
 // is 24.  An infinite or NaN input is laid out as 0 and its row marked; the
 // thread that joins such a row's sum adds those products itself, from A.
 //
+// 1x4096x65536 f16 26.4 us, 5.3 TB/s or 81% of a copy's rate; 8 rows 29.3 us (73%);
+// 1x4096x16384 f16 10.2 us and 1x640x640 f16 3.1 us, where start and join show.
+// 16 rows take 49 us: two MMAs a weight tile, and twice the columns to read from
+// shared memory.
+//
 // One CTA per SM walks the output tiles; A's rows are laid out in its shared
 // memory once.  Its warps split outputs (wm) and inputs (wk), so that the
 // outputs of an SM come out even: 1024 tiles on 148 SMs are 7 a SM, at once.

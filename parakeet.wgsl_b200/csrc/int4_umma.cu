@@ -19,8 +19,8 @@
 // 16x4096x65536 f32 59 us (mma.sync 86), 32x4096x65536 f16 66 us (94); reading
 // the codes takes 21.  Bound by instructions: about 470 per tile of 128 x 128
 // and SM sub-partition, of which expanding is a third (without the expansion 53
-// us where it takes 58, without seven of eight MMAs the same time, with an eighth
-// of the copies no less).  Register loads instead of bulk copies kept one
+// us where it takes 58, f32 54 of 59; with an eighth of the copies 57; with an
+// eighth of the MMAs the same time).  Register loads instead of bulk copies kept one
 // tile on the way whatever the depth asked for (58 us with two groups of
 // decode warps); MMAs issued behind `lane == 0` instead of an elected lane took
 // 85 cycles each instead of 20.

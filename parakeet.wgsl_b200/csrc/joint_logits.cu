@@ -18,6 +18,12 @@
 // instructions (with one thread doing both between barriers a step took 2400
 // cycles, 900 of them the MMAs' issue and 800 the loads').
 //
+// 1 window (61 tokens, 640 x 1032) f16 8.9 us: 17 tiles, latency from start to
+// end.  32 windows f16 12.0 us: 144 tiles, one per SM; reading everything once
+// takes 2.  40 windows f32 51 us, bound by shared memory: a step of 32 inputs
+// writes 64 KB of split operands there, reads 96 KB of them for its MMAs and
+// moves 32 KB of weights in and out, 1540 of its 2200 cycles.
+//
 // FP16: hidden is rounded to f16, as the decoder rounds its joint inputs; the
 // weight [inner, columns] arrives by TMA as it lies (the MN-major operand).
 // FP32: an f32 is the sum of two tf32 values up to 2^-22 of itself, so logits

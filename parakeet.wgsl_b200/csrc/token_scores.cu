@@ -27,7 +27,12 @@
 // warp, into which candidates are inserted one at a time.  Where fewer than K
 // columns are left by a mask, the lowest masked ids fill the places.
 //
-// Bound by reading the logits once.  A row belongs to one warp, to several
+// Bound by reading the logits once where rows are long and many, and there by
+// instructions on top: an element takes about ten (widen, compare, FMA, ex2, two
+// sums).  4096x50257 f16 103 us, 4.0 TB/s or 61% of a copy's rate (83 us without
+// alternatives); 16384x16384 f32 216 us, 5.0 TB/s.  Short calls are latency:
+// 1x32000 f16 6.3 us, 1953x1025 f32 6.4 us; a row of 8 columns takes 2.1.
+// A row belongs to one warp, to several
 // warps of a CTA or to a cluster of CTAs (joined through distributed shared
 // memory: no workspace, no atomics, so results do not depend on timing).
 #include <algorithm>
