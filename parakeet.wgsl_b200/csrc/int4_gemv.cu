@@ -501,7 +501,10 @@ int launch_int4_gemv(const DeviceCtx& dev, const pk_int4_gemv_desc& d, cudaStrea
   p.act = d.activation;
   p.residual_scale = d.residual_scale;
   p.status = dev.status;
-  if (umma_route(dev, p, d.precision == PK_FP16 ? 1 : 2)) return launch_int4_umma(dev, p, d.precision, (int)d.group, stream);
+  if (umma_route(dev, p, d.precision == PK_FP16 ? 1 : 2)) {
+    const int st = launch_int4_umma(dev, p, d.precision, (int)d.group, stream);
+    if (st != PK_E_SHAPE) return st;
+  }
   return d.precision == PK_FP16 ? launch_typed<__half>(dev, p, (int)d.group, stream)
                                 : launch_typed<float>(dev, p, (int)d.group, stream);
 }

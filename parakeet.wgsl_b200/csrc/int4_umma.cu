@@ -371,8 +371,8 @@ __global__ void __launch_bounds__(IU_THREADS, 1) int4_umma_kernel(const I4Params
       now.k += IU_PAIRS;
       now.settle(ktiles, walk);
     }
-    // After a wait that ran out: the MMAs issued are complete before TMEM is given back.
-    if (!good && leader) {
+    // The MMAs issued are complete before TMEM is given back, whoever gave up on them.
+    if (leader) {
       tc_commit(&drain[pair]);
       mbar_wait_drain(&drain[pair], 0, p.status);
     }
@@ -545,7 +545,7 @@ int launch_typed(const DeviceCtx& dev, I4Params p, int group, cudaStream_t strea
     }
     if (p.cluster <= I4_CLUSTER || cols <= 16) break;
   }
-  if (smem > I4_SMEM) return set_error(PK_E_SHAPE, "int4 products of K=%d do not fit shared memory", p.inner);
+  if (smem > I4_SMEM) return PK_E_SHAPE;
   int clusters = 0;
   const int st = int4_clusters(dev, p.cluster, &clusters);
   if (st != PK_OK) return st;
@@ -556,6 +556,7 @@ int launch_typed(const DeviceCtx& dev, I4Params p, int group, cudaStream_t strea
 
 }  // namespace
 
+// PK_E_SHAPE where even 16 columns of A do not fit a cluster's shared memory.
 int launch_int4_umma(const DeviceCtx& dev, const I4Params& p, int precision, int group, cudaStream_t stream) {
   return precision == PK_FP16 ? launch_typed<__half>(dev, p, group, stream) : launch_typed<float>(dev, p, group, stream);
 }

@@ -481,7 +481,7 @@ def test_int4_gemv(pk, device, profile, rows, inner, columns, group):
 @pytest.mark.parametrize("rows,inner,columns,group,epilogue", [
     (17, 1056, 12005, 32, "none"), (17, 640, 19000, 64, "bias"), (32, 4096, 4001, 128, "silu"), (33, 128, 97000, 128, "none"),
     (64, 8192, 1500, 512, "residual"), (20, 32768, 300, 128, "residual in place"), (19, 2208, 6100, 32, "relu"),
-    (64, 96, 50000, 32, "none"), (23, 16384, 1000, 64, "none"),
+    (64, 96, 50000, 32, "none"), (23, 16384, 1000, 64, "none"), (17, 65536, 260, 128, "none"), (33, 262144, 50, 4096, "none"),
 ])
 def test_int4_gemv_many_rows(pk, device, profile, rows, inner, columns, group, epilogue):
     _int4(pk, device, rows, inner, columns, group, profile, epilogue)
