@@ -32,10 +32,10 @@
 // is 24.  An infinite or NaN input is laid out as 0 and its row marked; the
 // thread that joins such a row's sum adds those products itself, from A.
 //
-// 1x4096x65536 f16 26.4 us, 5.3 TB/s or 81% of a copy's rate; 8 rows 29.3 us (73%);
-// 1x4096x16384 f16 10.2 us and 1x640x640 f16 3.1 us, where start and join show.
-// 16 rows take 49 us: two MMAs a weight tile, and twice the columns to read from
-// shared memory.
+// 1x4096x65536 f16 26.7 us, 5.2 TB/s or 80% of a copy's rate; 8 rows 30.2 us (71%);
+// 1x4096x16384 f16 10.6 us and 1x640x640 f16 3.2 us, where start and join show.
+// 16 rows take 51 us: two MMAs a weight tile, and twice the columns to read from
+// shared memory.  (What marks infinite inputs costs 0.1 to 0.4 us of these.)
 //
 // One CTA per SM walks the output tiles; A's rows are laid out in its shared
 // memory once.  Its warps split outputs (wm) and inputs (wk), so that the
@@ -440,7 +440,7 @@ int launch_typed(const DeviceCtx& dev, I4Params p, int group, cudaStream_t strea
 // (counted once per 32 columns).  Below that its pipeline is not filled, and its
 // tiles are too coarse to share out (32x1024x4096 f16: 8.3 us against 7.0 here);
 // above it, 32x4096x8192 f16 takes 15.0 us against 22.3, 64x4096x4096 21.5
-// against 27.1.  With 16 columns it is behind: 16x4096x65536 f16 55 us against 49.
+// against 27.1.  With 16 columns it is behind: 16x4096x65536 f16 55 us against 51.
 bool umma_route(const DeviceCtx& dev, const I4Params& p, int parts) {
   const int64_t columns = (int64_t)p.rows * parts, tiles = (int64_t)((p.columns + 127) / 128) * p.ktiles;
   return columns > 16 && tiles * ((columns + I4_COLS - 1) / I4_COLS) >= 5 * dev.sm_count;
