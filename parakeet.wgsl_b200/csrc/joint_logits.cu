@@ -11,18 +11,18 @@
 //
 // Both precisions run on the tensor cores (tcgen05, f32 accumulators in TMEM).
 // A tile is 128 rows times up to 256 (FP32: 128) columns, whose width follows
-// from the number of row tiles, so that few rows still fill the SMs.  8 warps (FP32: 16)
+// from the number of row tiles, so that few rows still fill the SMs.  16 warps
 // gather, add, clamp and lay out 128 bytes of inputs a step in shared memory
-// (K-major, 128-byte swizzle), their loads two steps ahead; one warp issues the
+// (K-major, 128-byte swizzle), their loads a step ahead; one warp issues the
 // MMAs, one the weights' loads, so that none of the three waits for another's
 // instructions (with one thread doing both between barriers a step took 2400
 // cycles, 900 of them the MMAs' issue and 800 the loads').
 //
-// 1 window (61 tokens, 640 x 1032) f16 8.9 us: 17 tiles, latency from start to
-// end.  32 windows f16 12.0 us: 144 tiles, one per SM; reading everything once
-// takes 2.  40 windows f32 51 us, bound by shared memory: a step of 32 inputs
+// 1 window (61 tokens, 640 x 1032) f16 8.4 us: 33 tiles, latency from start to
+// end.  32 windows f16 10.9 us: 144 tiles, one per SM; reading everything once
+// takes 2.  40 windows f32 48 us, bound by shared memory: a step of 32 inputs
 // writes 64 KB of split operands there, reads 96 KB of them for its MMAs and
-// moves 32 KB of weights in and out, 1540 of its 2200 cycles.
+// moves 32 KB of weights in and out, 1540 of its 2100 cycles.
 //
 // FP16: hidden is rounded to f16, as the decoder rounds its joint inputs; the
 // weight [inner, columns] arrives by TMA as it lies (the MN-major operand).
@@ -45,7 +45,7 @@
 namespace pk {
 namespace {
 
-constexpr int JL_ROWS = 512;       // threads that lay out rows and store logits, at most
+constexpr int JL_ROWS = 512;       // threads that lay out rows and store logits
 constexpr int JL_M = 128;          // rows per tile
 constexpr int JL_BAR = 192 * 1024;  // after the stages: the barriers
 constexpr int JL_MISC = JL_BAR + 256;
@@ -65,12 +65,7 @@ static_assert(JL_RAW == jl_stages<float>() * jl_stage<float>() && JL_RAW + JL_RA
 template <typename T>
 constexpr int jl_k() { return 128 / (int)sizeof(T); }  // inputs per step: 128 bytes
 constexpr int JL_TMEM = 512;       // TMEM columns: FP32's accumulators (FP16: 256 are enough)
-template <typename T>
-constexpr int jl_ahead() { return 2; }  // steps whose inputs are on their way to registers
-// Row threads: FP32 has the weights to lay out too.  A warp each for the MMAs
-// and the weights' loads comes after them.
-template <typename T>
-constexpr int jl_rows() { return sizeof(T) == 2 ? 256 : 512; }
+// Row threads.  A warp each for the MMAs and the weights' loads comes after them.
 template <typename T>
 constexpr int jl_n() { return sizeof(T) == 2 ? 256 : 128; }  // columns per tile, at most
 
@@ -171,29 +166,28 @@ __device__ __forceinline__ uint32_t jl_at(int r, int c) {
   return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
 }
 
-// What a thread gathers for one step: chunk tid % 8 of every 32nd (FP32: 64th) row.
-template <typename T>
-constexpr int jl_tasks() { return JL_M * 8 / jl_rows<T>(); }
+// What a thread gathers for one step: chunk tid % 8 of every 64th row.
+constexpr int JL_TASKS = JL_M * 8 / JL_ROWS;
 template <typename T>
 struct JlSlot;
 template <>
 struct JlSlot<__half> {
-  uint4 e[jl_tasks<__half>()];
-  float4 p[jl_tasks<__half>()][2];
+  uint4 e[JL_TASKS];
+  float4 p[JL_TASKS][2];
 };
 template <>
 struct JlSlot<float> {
-  float4 e[jl_tasks<float>()], p[jl_tasks<float>()];
+  float4 e[JL_TASKS], p[JL_TASKS];
 };
 
 template <typename T>
-__global__ void __launch_bounds__(jl_rows<T>() + 64, 1) joint_logits_kernel(const __grid_constant__ JlParams p) {
+__global__ void __launch_bounds__(JL_ROWS + 64, 1) joint_logits_kernel(const __grid_constant__ JlParams p) {
   pdl_entry();
   extern __shared__ uint8_t jl_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(jl_raw) + 1023) & ~uintptr_t(1023));
   __shared__ JlRows rows;
   constexpr bool F16 = sizeof(T) == 2;
-  constexpr int ROWS = jl_rows<T>(), TASKS = jl_tasks<T>();
+  constexpr int ROWS = JL_ROWS, TASKS = JL_TASKS;
   constexpr int K = jl_k<T>(), N = jl_n<T>(), EPC = 16 / sizeof(T);  // elements per chunk
   constexpr int STAGES = jl_stages<T>(), STAGE = jl_stage<T>(), B = jl_b<T>();
   constexpr int RAW = F16 ? STAGES : JL_RAW_STAGES;  // the weights' stages (FP16: the MMAs')
@@ -246,9 +240,9 @@ __global__ void __launch_bounds__(jl_rows<T>() + 64, 1) joint_logits_kernel(cons
   // Columns per tile, in units of 16: as few tiles as N columns allow, more while
   // SMs are idle.  FP16 shares the units out evenly.  FP32 fills its tiles: the 8
   // columns that 1032 leave to a ninth one cost less there than nine equal tiles
-  // (and less than a 144-column tile among eight: 40 windows 51 against 54 us).
+  // (and less than a 144-column tile among eight: 40 windows 54 against 51 us).
   const int units = (p.columns + 15) / 16;
-  int ntiles = max((units + N / 16 - 1) / (N / 16), min((p.columns + 63) / 64, (int)gridDim.x / max(mtiles, 1)));
+  int ntiles = max((units + N / 16 - 1) / (N / 16), min((p.columns + 31) / 32, (int)gridDim.x / max(mtiles, 1)));
   const int even = units / ntiles, rest = units % ntiles, most = even + (rest > 0 ? 1 : 0);
   if (!F16) ntiles = (units + most - 1) / most;
   auto tile_start = [&](int t) { return 16 * (F16 ? t * even + min(t, rest) : t * most); };
@@ -368,72 +362,64 @@ __global__ void __launch_bounds__(jl_rows<T>() + 64, 1) joint_logits_kernel(cons
           }
         }
       };
-      constexpr int AHEAD = jl_ahead<T>();
-      JlSlot<T> slot[AHEAD];
+      // One step ahead: with the loads of two in registers a step waits for the
+      // younger ones too (32 windows f16 10.9 us, with two 12.0).
+      JlSlot<T> s;
+      fetch(s, 0);
+      for (int kb = 0; kb < steps; ++kb) {
+        const uint32_t st = used % STAGES, use = used / STAGES;
+        uint8_t* stage = sm + st * STAGE;
+        if (use > 0 && good) good = mbar_wait(&empty[st], (use - 1) & 1, abort_flag, p.status, PK_STATUS_TIMEOUT_MMA);
+        if (!F16 && good) good = mbar_wait(&weights[used % RAW], used / RAW & 1, abort_flag, p.status, PK_STATUS_TIMEOUT_TMA);
+        good = __all_sync(0xffffffffu, good);
+        if (good) {
 #pragma unroll
-      for (int d = 0; d < AHEAD; ++d)
-        if (d < steps) fetch(slot[d], d);
-      for (int kb0 = 0; kb0 < steps; kb0 += AHEAD) {
-#pragma unroll
-        for (int d = 0; d < AHEAD; ++d) {
-          const int kb = kb0 + d;
-          if (kb < steps) {
-            const uint32_t st = used % STAGES, use = used / STAGES;
-            uint8_t* stage = sm + st * STAGE;
-            if (use > 0 && good) good = mbar_wait(&empty[st], (use - 1) & 1, abort_flag, p.status, PK_STATUS_TIMEOUT_MMA);
-            if (!F16 && good) good = mbar_wait(&weights[used % RAW], used / RAW & 1, abort_flag, p.status, PK_STATUS_TIMEOUT_TMA);
-            good = __all_sync(0xffffffffu, good);
-            JlSlot<T>& s = slot[d];
-            if (good) {
-#pragma unroll
-              for (int i = 0; i < TASKS; ++i) {
-                const uint32_t at = jl_at(rbase + ROWS / 8 * i, chunk);
-                if constexpr (F16) {
-                  uint4 o;
-                  o.x = jl_hidden2(s.e[i].x, s.p[i][0].x, s.p[i][0].y);
-                  o.y = jl_hidden2(s.e[i].y, s.p[i][0].z, s.p[i][0].w);
-                  o.z = jl_hidden2(s.e[i].z, s.p[i][1].x, s.p[i][1].y);
-                  o.w = jl_hidden2(s.e[i].w, s.p[i][1].z, s.p[i][1].w);
-                  *reinterpret_cast<uint4*>(stage + at) = o;
-                } else {
-                  uint4 hi, lo;
-                  jl_split(jl_relu(s.e[i].x + s.p[i].x), hi.x, lo.x);
-                  jl_split(jl_relu(s.e[i].y + s.p[i].y), hi.y, lo.y);
-                  jl_split(jl_relu(s.e[i].z + s.p[i].z), hi.z, lo.z);
-                  jl_split(jl_relu(s.e[i].w + s.p[i].w), hi.w, lo.w);
-                  *reinterpret_cast<uint4*>(stage + at) = hi;
-                  *reinterpret_cast<uint4*>(stage + JL_M * 128 + at) = lo;
-                }
-              }
-              if constexpr (!F16) {
-                const float* raw = reinterpret_cast<const float*>(sm + JL_RAW + used % RAW * JL_RAW_STAGE) + wn;
-                if (wn < bn) {
-#pragma unroll
-                  for (int i = 0; i < K / 16; ++i) {  // 16 inputs at a time over the row threads
-                    float w[4];
-                    uint4 hi, lo;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) w[j] = raw[(4 * wk + 16 * i + j) * N];
-                    jl_split(w[0], hi.x, lo.x);
-                    jl_split(w[1], hi.y, lo.y);
-                    jl_split(w[2], hi.z, lo.z);
-                    jl_split(w[3], hi.w, lo.w);
-                    const uint32_t wat = jl_at(wn, wk + 4 * i);
-                    *reinterpret_cast<uint4*>(stage + B + wat) = hi;
-                    *reinterpret_cast<uint4*>(stage + B + N * 128 + wat) = lo;
-                  }
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&unpacked[used % RAW]);
-              }
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&full[st]);
+          for (int i = 0; i < TASKS; ++i) {
+            const uint32_t at = jl_at(rbase + ROWS / 8 * i, chunk);
+            if constexpr (F16) {
+              uint4 o;
+              o.x = jl_hidden2(s.e[i].x, s.p[i][0].x, s.p[i][0].y);
+              o.y = jl_hidden2(s.e[i].y, s.p[i][0].z, s.p[i][0].w);
+              o.z = jl_hidden2(s.e[i].z, s.p[i][1].x, s.p[i][1].y);
+              o.w = jl_hidden2(s.e[i].w, s.p[i][1].z, s.p[i][1].w);
+              *reinterpret_cast<uint4*>(stage + at) = o;
+            } else {
+              uint4 hi, lo;
+              jl_split(jl_relu(s.e[i].x + s.p[i].x), hi.x, lo.x);
+              jl_split(jl_relu(s.e[i].y + s.p[i].y), hi.y, lo.y);
+              jl_split(jl_relu(s.e[i].z + s.p[i].z), hi.z, lo.z);
+              jl_split(jl_relu(s.e[i].w + s.p[i].w), hi.w, lo.w);
+              *reinterpret_cast<uint4*>(stage + at) = hi;
+              *reinterpret_cast<uint4*>(stage + JL_M * 128 + at) = lo;
             }
-            if (kb + AHEAD < steps) fetch(s, kb + AHEAD);
-            ++used;
           }
+          if constexpr (!F16) {
+            const float* raw = reinterpret_cast<const float*>(sm + JL_RAW + used % RAW * JL_RAW_STAGE) + wn;
+            if (wn < bn) {
+#pragma unroll
+              for (int i = 0; i < K / 16; ++i) {  // 16 inputs at a time over the row threads
+                float w[4];
+                uint4 hi, lo;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = raw[(4 * wk + 16 * i + j) * N];
+                jl_split(w[0], hi.x, lo.x);
+                jl_split(w[1], hi.y, lo.y);
+                jl_split(w[2], hi.z, lo.z);
+                jl_split(w[3], hi.w, lo.w);
+                const uint32_t wat = jl_at(wn, wk + 4 * i);
+                *reinterpret_cast<uint4*>(stage + B + wat) = hi;
+                *reinterpret_cast<uint4*>(stage + B + N * 128 + wat) = lo;
+              }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&unpacked[used % RAW]);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[st]);
         }
+        if (kb + 1 < steps) fetch(s, kb + 1);
+        ++used;
       }
       if (good) good = mbar_wait(done, turn & 1, abort_flag, p.status, PK_STATUS_TIMEOUT_EPILOGUE);
       good = __all_sync(0xffffffffu, good);
@@ -496,9 +482,9 @@ template <typename T>
 int launch_typed(const DeviceCtx& dev, const JlParams& p, cudaStream_t stream) {
   const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(joint_logits_kernel<T>), JL_SMEM);
   if (st != PK_OK) return st;
-  const int64_t tiles = ((int64_t)p.batch * p.max_tokens + JL_M - 1) / JL_M * ((p.columns + 63) / 64);
+  const int64_t tiles = ((int64_t)p.batch * p.max_tokens + JL_M - 1) / JL_M * ((p.columns + 31) / 32);
   return cuda_error(launch_kernel(joint_logits_kernel<T>, dim3((unsigned)std::min<int64_t>(tiles, dev.sm_count)),
-                                  dim3(jl_rows<T>() + 64), JL_SMEM, stream, p),
+                                  dim3(JL_ROWS + 64), JL_SMEM, stream, p),
                     "joint_logits launch");
 }
 
