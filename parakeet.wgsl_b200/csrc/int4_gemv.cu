@@ -32,8 +32,8 @@
 // is 24.  An infinite or NaN input is laid out as 0 and its row marked; the
 // thread that joins such a row's sum adds those products itself, from A.
 //
-// 1x4096x65536 f16 26.7 us, 5.2 TB/s or 80% of a copy's rate; 8 rows 30.2 us (71%);
-// 1x4096x16384 f16 10.6 us and 1x640x640 f16 3.2 us, where start and join show.
+// 1x4096x65536 f16 26.7 us, 5.2 TB/s or 80% of a copy's rate; 8 rows 29.9 us (72%);
+// 1x4096x16384 f16 10.1 us and 1x640x640 f16 3.0 us, where start and join show.
 // 16 rows take 51 us: two MMAs a weight tile, and twice the columns to read from
 // shared memory.  (What marks infinite inputs costs 0.1 to 0.4 us of these.)
 //
@@ -62,7 +62,7 @@ constexpr int I4_COLS = 32;       // columns of one pass, at most (more rows: th
 // us; with 32 columns their sums leave room for 12 warps alone, 86 -> 92 us.
 __host__ __device__ constexpr int i4_warps(int nt) { return nt == 1 ? 28 : 16; }
 __host__ __device__ constexpr int i4_mt(int nt) { return nt == 2 ? 2 : 1; }
-__host__ __device__ constexpr int i4_depth(int nt) { return nt == 2 ? 2 : 3; }
+__host__ __device__ constexpr int i4_depth(int nt) { return nt == 4 ? 3 : 2; }
 
 // Eight codes -> the pairs (0,4) (2,6) of code - 8 and (1,5) (3,7) of code + 64.
 __device__ __forceinline__ void i4_expand(uint32_t w, uint32_t (&p)[4]) {
@@ -406,8 +406,11 @@ int launch_typed(const DeviceCtx& dev, I4Params p, int group, cudaStream_t strea
   for (;; cols = std::max(PARTS, cols / 2 / PARTS * PARTS)) {
     p.rows_per_pass = cols / PARTS;
     nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-    const int mt = i4_mt(nt), warps = i4_warps(nt);
+    const int mt = i4_mt(nt);
     mgroups = (mtiles + mt - 1) / mt;
+    // Few tiles per SM: fewer warps to start and to join (8x4096x4096 f16 7.3 us
+    // with 20 against 8.0; at 221 tiles per SM, 1x4096x16384, 12.2 against 10.1).
+    const int warps = nt == 1 && (int64_t)mgroups * p.ktiles < 100 * dev.sm_count ? 20 : i4_warps(nt);
     for (p.cluster = 1; p.cluster <= I4_CLUSTER; p.cluster *= 2) {
       // Few outputs: the inputs over more SMs, while each has a tile for every warp of 4.
       if (mgroups * p.cluster * 2 <= dev.sm_count && p.cluster < I4_CLUSTER && p.ktiles >= p.cluster * 2 * 4) continue;
