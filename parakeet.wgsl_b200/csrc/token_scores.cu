@@ -7,8 +7,10 @@
 // and the K best (value, then lower index) with their d - log s.  The sums run
 // in base 2: t_j = x_j L - b with L = log2(e) as rounded and b = m L rounded is
 // one FMA, and exact up to its own rounding; b's rounding r = m L - b shifts
-// every t alike and is taken out at the end.  Parts of a row with bases b and
-// b + g join as s 2^{-g}, (u - g s) 2^{-g}.  Statistics are f32 whatever the
+// every t alike and is taken out at the end.  r grows with m, so beyond 2^16
+// (which no f16 reaches), where it is 2^-8, t_j = (x_j - m) L takes its place,
+// with b = r = 0: a logit may be any finite number.  Parts of a row with bases b
+// and b + g join as s 2^{-g}, (u - g s) 2^{-g}.  Statistics are f32 whatever the
 // logits' type.  A masked (-inf) logit has t clamped, to where 2^t is zero, so
 // that it adds 0 to u and not 0 * -inf; the clamp passes NaN on.  A row with a
 // NaN or a +inf has no distribution: its numbers are NaN, its alternatives
@@ -29,9 +31,9 @@
 //
 // Bound by reading the logits once where rows are long and many, and there by
 // instructions on top: an element takes about ten (widen, compare, FMA, ex2, two
-// sums).  4096x50257 f16 103 us, 4.0 TB/s or 61% of a copy's rate (83 us without
-// alternatives); 16384x16384 f32 216 us, 5.0 TB/s.  Short calls are latency:
-// 1x32000 f16 6.3 us, 1953x1025 f32 6.4 us; a row of 8 columns takes 2.1.
+// sums).  4096x50257 f16 100 us, 4.1 TB/s or 63% of a copy's rate (80 us without
+// alternatives); 16384x16384 f32 218 us, 4.9 TB/s.  Short calls are latency:
+// 1x32000 f16 5.7 us, 1953x1025 f32 6.4 us; a row of 8 columns takes 3.1.
 // A row belongs to one warp, to several
 // warps of a CTA or to a cluster of CTAs (joined through distributed shared
 // memory: no workspace, no atomics, so results do not depend on timing).
@@ -57,6 +59,7 @@ constexpr int TS_POOL = 128;             // candidates per warp of a row
 constexpr uint32_t TS_MASKED = 0x007fffffu;  // ts_ordered(-inf)
 constexpr float TS_LOG2E = 1.4426950408889634f;
 constexpr float TS_LN2 = 0.6931471805599453f;
+constexpr float TS_FAR = 65536.0f;  // beyond: t from x - m
 
 struct TsParams {
   const void* logits;
@@ -113,12 +116,25 @@ __device__ __forceinline__ uint64_t ts_key(float v, uint32_t id) {
   return (uint64_t)ts_ordered(v != v ? -INFINITY : v) << 32 | (uint32_t)~id;
 }
 
-// The factor of x in t (beyond 1e37, where x L could overflow, neighbouring
-// values are so far apart that any factor gives 2^t = 0 or 1) and the base.
-__device__ __forceinline__ float ts_factor(float m) { return fabsf(m) <= 1e37f ? TS_LOG2E : 1.0f; }
-__device__ __forceinline__ float ts_base(float m) { return m > -INFINITY ? __fmul_rn(m, ts_factor(m)) : 0.0f; }
+// Whether t is (x - m) L, the base of a maximum, and what its rounding leaves of
+// m L.  A part whose maximum is -inf holds masked logits or NaN alone.
+__device__ __forceinline__ bool ts_far(float m) { return fabsf(m) > TS_FAR && fabsf(m) < INFINITY; }
+template <typename T>
+__device__ __forceinline__ float ts_base(float m) {
+  return m > -INFINITY && !(sizeof(T) == 4 && ts_far(m)) ? __fmul_rn(m, TS_LOG2E) : 0.0f;
+}
+template <typename T>
+__device__ __forceinline__ float ts_rest(float m) {
+  return sizeof(T) == 4 && ts_far(m) ? 0.0f : fmaf(m, TS_LOG2E, -ts_base<T>(m));
+}
+// The power of 2 that takes sums of maximum a (base ab) to maximum b (base bb).
+template <typename T>
+__device__ __forceinline__ float ts_gap(float a, float ab, float b, float bb) {
+  if (sizeof(T) == 4 && (ts_far(a) || ts_far(b))) return fmaf(a - b, TS_LOG2E, ts_rest<T>(b) - ts_rest<T>(a));
+  return ab - bb;
+}
 
-// (s, u) of base b rescaled to a base that is larger by -g.
+// (s, u) times 2^g, with t less by -g.
 __device__ __forceinline__ void ts_shift(float g, float& s, float& u) {
   const float c = ts_ex2(g);
   u = c == 0.0f ? 0.0f : c * fmaf(g, s, u);  // once 2^g is 0 nothing is left
@@ -132,26 +148,26 @@ __device__ __forceinline__ void ts_shift(float g, float2& s, float2& u) {
   u = ffma2(ffma2(s, make_float2(d, d), u), c2, zero);
   s = ffma2(s, c2, zero);
 }
-__device__ __forceinline__ TsStat ts_join(TsStat a, TsStat b) {
-  TsStat r{fmaxf(a.m, b.m), 0.0f, 0.0f};
-  auto add = [&](TsStat p) {
-    if (p.s == 0.0f) return;  // nothing but masked logits
-    if (p.m != r.m) ts_shift(ts_base(p.m) - ts_base(r.m), p.s, p.u);
-    r.s += p.s;
-    r.u += p.u;
-  };
-  add(a);
-  add(b);
-  return r;
-}
 
 // The sums of the `n` (at most 8) parts of a row, in their order.
-__device__ __forceinline__ TsStat ts_join_warps(const TsStat* part, int n) {
-  TsStat st = part[0];
+template <typename T>
+__device__ __forceinline__ TsStat ts_join(const TsStat* part, int n) {
+  TsStat r = part[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i)
-    if (i < n) st = ts_join(st, part[i]);
-  return st;
+    if (i < n) r.m = fmaxf(r.m, part[i].m);
+  const float base = ts_base<T>(r.m);
+  r.s = r.u = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (i >= n) continue;
+    TsStat p = part[i];
+    if (p.s == 0.0f) continue;  // nothing but masked logits
+    ts_shift(p.m == r.m ? 0.0f : ts_gap<T>(p.m, ts_base<T>(p.m), r.m, base), p.s, p.u);
+    r.s += p.s;
+    r.u += p.u;
+  }
+  return r;
 }
 
 // N 16-byte vectors of a row per lane.
@@ -211,10 +227,11 @@ struct TsTile {
     }
   }
   __device__ __forceinline__ float maximum() const { return largest(raw, N); }
-  // s += sum 2^t, u += sum 2^t t for t = x a - base (of the maximum m).
-  __device__ __forceinline__ void sums(float m, float a, float base, float2& s, float2& u) const {
+  // s += sum 2^t, u += sum 2^t t, relative to the maximum m of that base (FAR: of any size).
+  template <bool FAR = sizeof(T) == 4>
+  __device__ __forceinline__ void sums(float m, float base, float2& s, float2& u) const {
     const float b = -base;
-    const float2 a2 = make_float2(a, a), b2 = make_float2(b, b), one = make_float2(1.0f, 1.0f);
+    const float2 a2 = make_float2(TS_LOG2E, TS_LOG2E), b2 = make_float2(b, b), one = make_float2(1.0f, 1.0f);
     auto add = [&](float2 t) {
       const float2 e = make_float2(ts_ex2(t.x), ts_ex2(t.y));
       s = ffma2(e, one, s);
@@ -234,22 +251,32 @@ struct TsTile {
         return;
       }
     }
-    auto clamped = [&](float2 x) {
-      float2 t = ffma2(x, a2, b2);
+    auto clamp = [&](float2 t) {
       t.x = ts_max_nan(t.x, -300.0f);
       t.y = ts_max_nan(t.y, -300.0f);
       add(t);
     };
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int q = 0; q < N; ++q) {
-      if constexpr (sizeof(T) == 2) {
+      for (int q = 0; q < N; ++q) {
         const __half2* h = reinterpret_cast<const __half2*>(&raw[q]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) clamped(__half22float2(h[j]));
-      } else {
+        for (int j = 0; j < 4; ++j) clamp(ffma2(__half22float2(h[j]), a2, b2));
+      }
+    } else if (!FAR || !ts_far(m)) {
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
         const float2* h = reinterpret_cast<const float2*>(&raw[q]);
-        clamped(h[0]);
-        clamped(h[1]);
+        clamp(ffma2(h[0], a2, b2));
+        clamp(ffma2(h[1], a2, b2));
+      }
+    } else {
+      const float2 m2 = make_float2(-m, -m), zero = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        const float2* h = reinterpret_cast<const float2*>(&raw[q]);
+        clamp(ffma2(ffma2(h[0], one, m2), a2, zero));
+        clamp(ffma2(ffma2(h[1], one, m2), a2, zero));
       }
     }
   }
@@ -411,7 +438,7 @@ __global__ void __launch_bounds__(TS_THREADS, sizeof(T) == 2 && NV > 0 ? (NV == 
     const float mine = tile.maximum();
     st.m = ts_value(__reduce_max_sync(0xffffffffu, ts_ordered(mine)));
     float2 s2 = make_float2(0.0f, 0.0f), u2 = make_float2(0.0f, 0.0f);
-    tile.sums(st.m, ts_factor(st.m), ts_base(st.m), s2, u2);
+    tile.sums(st.m, ts_base<T>(st.m), s2, u2);
     st.s = s2.x + s2.y;
     st.u = u2.x + u2.y;
 #pragma unroll
@@ -459,17 +486,16 @@ __global__ void __launch_bounds__(TS_THREADS, sizeof(T) == 2 && NV > 0 ? (NV == 
   } else {
     const int step = warps * 32 * TS_UNR, first = gw * 32 * TS_UNR;
     float2 s2 = make_float2(0.0f, 0.0f), u2 = make_float2(0.0f, 0.0f);
-    float m = -INFINITY, ma = TS_LOG2E, mb = 0.0f;  // the maximum, its factor and base
+    float m = -INFINITY, mb = 0.0f;  // the maximum and its base
     auto take = [&](const TsTile<T, TS_UNR>& tile) {
       const float tm = tile.maximum();
       if (tm > m) {
-        const float to = ts_base(tm);
+        const float to = ts_base<__half>(tm);
         if (m > -INFINITY) ts_shift(mb - to, s2, u2);
         m = tm;
-        ma = ts_factor(tm);
         mb = to;
       }
-      tile.sums(m, ma, mb, s2, u2);
+      tile.template sums<false>(m, mb, s2, u2);
     };
     // The warps of four CTAs an SM cover each other's loads (a second tile in
     // registers, loaded ahead, was 7% slower: fewer warps, more moves).
@@ -478,9 +504,22 @@ __global__ void __launch_bounds__(TS_THREADS, sizeof(T) == 2 && NV > 0 ? (NV == 
       tile.load(base, skew, columns, v, lane, 32, vectors);
       take(tile);
     }
+    // Every maximum was taken to be within 2^16: others leave sums that are not
+    // finite or are multiplied by zero, unless the last is one of them.  Such rows
+    // are read again with the maxima known (to ask before each tile took 3%).
+    if constexpr (sizeof(T) == 4) {
+      if (__any_sync(0xffffffffu, ts_far(m) || !(fabsf(s2.x + s2.y + u2.x + u2.y) < INFINITY))) {
+        mb = ts_base<T>(m);
+        s2 = u2 = make_float2(0.0f, 0.0f);
+        for (int v = first; v < vectors; v += step) {
+          tile.load(base, skew, columns, v, lane, 32, vectors);
+          tile.sums(m, mb, s2, u2);
+        }
+      }
+    }
     // The lanes' sums, brought to the warp's maximum.
     st = TsStat{ts_value(__reduce_max_sync(0xffffffffu, ts_ordered(m))), s2.x + s2.y, u2.x + u2.y};
-    if (st.s != 0.0f && m != st.m) ts_shift(mb - ts_base(st.m), st.s, st.u);
+    if (st.s != 0.0f && m != st.m) ts_shift(ts_gap<T>(m, mb, st.m, ts_base<T>(st.m)), st.s, st.u);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
@@ -566,7 +605,7 @@ __global__ void __launch_bounds__(TS_THREADS, sizeof(T) == 2 && NV > 0 ? (NV == 
   if constexpr (CLUSTER) {
     __syncthreads();  // the warps' sums
     if (tid == 0) {
-      st = ts_join_warps(sm.stat, TS_WARPS);
+      st = ts_join<T>(sm.stat, TS_WARPS);
       const uint32_t cs = mapa_shared(smem_addr(&sm.cstat[rank]), 0);
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cs), "f"(st.m) : "memory");
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cs + 4), "f"(st.s) : "memory");
@@ -583,10 +622,10 @@ __global__ void __launch_bounds__(TS_THREADS, sizeof(T) == 2 && NV > 0 ? (NV == 
   }
   if (k > 0 || wpr > 1) ts_row_sync(group, wpr);
   if (!live || wig != 0) return;
-  if constexpr (CLUSTER) st = ts_join_warps(sm.cstat, ranks);
-  else if (wpr > 1) st = ts_join_warps(sm.stat + group * wpr, wpr);
+  if constexpr (CLUSTER) st = ts_join<T>(sm.cstat, ranks);
+  else if (wpr > 1) st = ts_join<T>(sm.stat + group * wpr, wpr);
   const bool empty = st.s == 0.0f;
-  const float r = fmaf(st.m, ts_factor(st.m), -ts_base(st.m)) * TS_LN2;  // the base's rounding
+  const float r = ts_rest<T>(st.m) * TS_LN2;  // the base's rounding
   const float log_s = empty ? 0.0f : logf(st.s) - r;
   if (lane == 0) {
     if (p.log_probs) p.log_probs[slot] = empty ? (given == given ? -INFINITY : NAN) : (given - st.m) - log_s;

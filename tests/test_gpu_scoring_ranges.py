@@ -1,0 +1,112 @@
+"""The scoring operators on numbers far from one: large finite logits.
+
+E = 2^-24 is half a step of f32 arithmetic, relative."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from test_gpu_scoring import E, Scores, _logits, _score_reference
+
+pytestmark = pytest.mark.gpu
+
+
+# ====================================================================== token scores
+
+MASKS = {"fp16": (-300.0, -1e4, -6e4, -65504.0),
+         "fp32": (-300.0, -1e4, -65535.0, -65537.0, -1e5, -1e9, -1e10, -1e20, -1e30, -0.9e37, -1e37, -1.1e37,
+                  float(np.finfo(np.float32).min))}
+PEAKS = {"fp16": (300.0, 2e4, 65504.0),
+         "fp32": (300.0, 65535.0, 65537.0, 1e5, 1e9, 1e10, 1e20, 1e30, 0.9e37, 1e37, 1.1e37, float(np.finfo(np.float32).max) / 2)}
+
+
+def _wide_rows(rng, columns, profile):
+    """Rows with finite masks and peaks of every size, ties of them, values of all sizes and rows about 2^16."""
+    dt = np.float16 if profile == "fp16" else np.float32
+    base = lambda: _logits(rng, 1, columns, profile)[0].astype(np.float64)  # noqa: E731
+    rows = []
+    for m in MASKS[profile]:
+        for share in (0.5, 0.95):
+            x = base()
+            x[:int(share * columns)] = m  # a contiguous part: whole warps see nothing else
+            rows.append(x)
+        x = base()
+        x[rng.random(columns) < 0.95] = m
+        rows.append(x)
+        rows.append(np.full(columns, m))
+        x = np.full(columns, m)
+        x[columns // 3] = 1.5
+        rows.append(x)
+        x = np.full(columns, m)
+        x[::2] = -np.inf
+        rows.append(x)
+    for p in PEAKS[profile]:
+        x = base()
+        x[columns // 5] = p
+        rows.append(x)
+        x = base()
+        x[[columns // 7, columns - 1]] = p  # a tie, in different warps
+        rows.append(x)
+        x = base()
+        x[columns - 1], x[0] = p, 0.9 * p  # two sizes in different warps
+        rows.append(x)
+        x = base()
+        x[0], x[columns - 1] = p, 0.9 * p
+        rows.append(x)
+    top = 4.0 if profile == "fp16" else 37.0
+    for sign in (-1.0, 1.0):
+        rows.append(sign * 10.0 ** rng.uniform(-3, top, columns))
+        rows.append(sign * np.sort(10.0 ** rng.uniform(-3, top, columns)))
+        middle = 60000.0 if profile == "fp16" else 65536.0
+        rows.append(sign * middle + base() * (8.0 if profile == "fp16" else 0.5))  # neighbours about 2^16
+        rows.append(sign * middle + np.sort(base()) * (8.0 if profile == "fp16" else 0.5))
+    return np.array(rows).astype(dt)
+
+
+@pytest.mark.parametrize("profile", ["fp16", "fp32"])
+@pytest.mark.parametrize("rows,columns,k", [
+    (0, 2, 0), (0, 200, 4), (0, 1999, 8), (0, 9001, 5), (2600, 1025, 4), (1300, 9000, 3),
+])
+def test_token_scores_of_large_finite_logits(pk, device, profile, rows, columns, k):
+    """Held by one warp and by several, streamed by one warp and by several (`rows` at least in one call)."""
+    x = _wide_rows(np.random.default_rng(71 + columns), columns, profile)
+    _check_wide(pk, device, np.resize(x, (max(rows, len(x)), columns)), len(x), columns, k, profile)
+
+
+@pytest.mark.parametrize("profile", ["fp16", "fp32"])
+@pytest.mark.parametrize("columns", [20000, 131075])
+def test_token_scores_of_large_finite_logits_over_clusters(pk, device, profile, columns):
+    """A row over a cluster of CTAs, held and streamed: three rows a call."""
+    x = _wide_rows(np.random.default_rng(72 + columns), columns, profile)
+    for r in range(0, len(x), 3):
+        _check_wide(pk, device, x[r:r + 3], len(x[r:r + 3]), columns, 4, profile)
+
+
+def _check_wide(pk, device, x, n, columns, k, profile):
+    import torch
+
+    rng = np.random.default_rng(5)
+    targets = rng.integers(0, columns, len(x))
+    targets[::2] = x[::2].argmax(axis=1)
+    got = Scores(pk, device, torch.from_numpy(x).cuda(), columns, profile, torch.from_numpy(targets.astype(np.int32)).cuda(),
+                 k)().host()
+    got = {name: v[:n].astype(np.float64) for name, v in got.items()}
+    ref = _score_reference(x[:n].astype(np.float64) + 0.0, targets[:n], k)
+    np.testing.assert_array_equal(got["top_ids"], ref["top_ids"])
+    # d = x - m, its product with log2 e and the exponential round at their own sizes: e^d is off by
+    # e^d (|d| 3 E + 4 E) at most, of which |d| e^d <= 1/e, so s by under 6 E of itself, beside its sums (a thread's
+    # chain of columns / 32 terms at most, and the joins).  log p = d - log s and log sum = m + log s round at their
+    # own sizes; no error grows with the logits.
+    rel = (columns / 32 + 64) * E
+    for name in ("log_probs", "log_sums", "top_log_probs"):
+        g, r = got[name], ref[name]
+        gone = np.isneginf(r)
+        np.testing.assert_array_equal(np.isneginf(g), gone, err_msg=name)
+        g, r = np.where(gone, 0.0, g), np.where(gone, 0.0, r)
+        bad = ~(np.abs(g - r) <= rel + 4 * E * np.abs(r))
+        assert not bad.any(), (name, np.argwhere(bad)[:5].tolist(), g[bad][:5], r[bad][:5])
+    # u = sum e^d d, relative to s: its terms' errors are |d| times those of the exponentials, and |u| / s is
+    # log s - entropy, below log columns.
+    g, r, span = got["entropies"], ref["entropies"], np.log(columns)
+    bad = ~(np.abs(g - r) <= rel * (4 + 2 * span))
+    assert not bad.any(), ("entropies", np.argwhere(bad)[:5].tolist(), g[bad][:5], r[bad][:5])
