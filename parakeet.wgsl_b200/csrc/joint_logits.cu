@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(JL_ROWS + 64, 1) joint_logits_kernel(const __g
   uint64_t* empty = unpacked + RAW;                           // the stage's MMAs have read it
   uint64_t* done = empty + STAGES;                            // the tile's MMAs are complete
   uint64_t* taken = done + 1;                                 // the tile's accumulators are read
+  uint64_t* drain = taken + 1;                                // every MMA issued is complete
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + JL_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + JL_MISC + 4);
   int* totals = reinterpret_cast<int*>(sm + JL_MISC + 8);
@@ -212,6 +213,7 @@ __global__ void __launch_bounds__(JL_ROWS + 64, 1) joint_logits_kernel(const __g
     }
     mbar_init(done, 1);
     mbar_init(taken, ROWS / 32);
+    mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&p.tmap_w);
@@ -295,8 +297,10 @@ __global__ void __launch_bounds__(JL_ROWS + 64, 1) joint_logits_kernel(const __g
         }
         if (good) tc_commit(done);
       }
-      // Unwind: the MMAs issued are complete before the roles meet.
-      if (!good && used > 0) mbar_wait_drain(&empty[(used - 1) % STAGES], (used - 1) / STAGES & 1, p.status);
+      // The MMAs issued are complete before the roles meet and TMEM is given back, whoever gave up on them: a row
+      // warp's wait may expire where none of this thread's did.
+      tc_commit(drain);
+      mbar_wait_drain(drain, 0, p.status);
     }
   } else if (warp == ROWS / 32 + 1) {
     // ------------------------------------------------------------ weights
