@@ -277,7 +277,9 @@ int pk_token_scores(pk_device* device, const pk_token_scores_desc* desc, pk_stre
  *   u = post(block), y = input + residual_scale * gate * u, h = pre(y)
  * where post and pre are PK_NORM_*; y (output) and h (normalized) are each
  * rounded once, h from the unrounded y.  LayerNorm has gamma and beta, RMS
- * norm gamma alone.  gate: NULL, or f32 [ceil(rows / gate_rows), channels]
+ * norm gamma alone.  Statistics are f32: where a mean square is infinite there
+ * (a value is, or its square beyond 3e38), the row's finite values become 0
+ * before gamma, its infinite ones NaN.  gate: NULL, or f32 [ceil(rows / gate_rows), channels]
  * (one row for each gate_rows rows; gate_rows 0: one row for all).  output
  * and normalized may take the place of input or block (exactly), not of each
  * other. */

@@ -97,10 +97,11 @@ __device__ __forceinline__ void rn_params(const float* src, float (&v)[VEC]) {
   }
 }
 
-// 1 / sqrt(v): the hardware's estimate (2 ulp) and one Newton step.
+// 1 / sqrt(v): the hardware's estimate (2 ulp) and one Newton step, where neither
+// v nor the result is infinite (the step would meet inf * 0).
 __device__ __forceinline__ float rn_rsqrt(float v) {
   const float r = rsqrtf(v);
-  return fmaf(r * 0.5f, fmaf(-v * r, r, 1.0f), r);
+  return r > 0.0f && r < INFINITY ? fmaf(r * 0.5f, fmaf(-v * r, r, 1.0f), r) : r;
 }
 
 // Sum over the G threads of a row.  Rows of more than a warp meet in shared

@@ -110,3 +110,58 @@ def _check_wide(pk, device, x, n, columns, k, profile):
     g, r, span = got["entropies"], ref["entropies"], np.log(columns)
     bad = ~(np.abs(g - r) <= rel * (4 + 2 * span))
     assert not bad.any(), ("entropies", np.argwhere(bad)[:5].tolist(), g[bad][:5], r[bad][:5])
+
+
+# ====================================================================== residual norm
+
+@pytest.mark.parametrize("profile", ["fp16", "fp32"])
+@pytest.mark.parametrize("channels", [64, 1000, 1002 * 4, 9000, 32768])
+@pytest.mark.parametrize("unaligned", [False, True])
+def test_residual_norm_of_rows_whose_squares_leave_f32(pk, device, profile, channels, unaligned):
+    """The mean square is infinite where a value is, or where its square is in f32: finite values over its root are
+    0, by the formula, an infinite one is NaN, and the rows beside keep what they have alone."""
+    import torch
+
+    dt = torch.float16 if profile == "fp16" else torch.float32
+    rng = np.random.default_rng(channels)
+    x, f = (_logits(rng, 6, channels, profile, 1.0) for _ in range(2))
+    f[1, 7] = np.inf
+    x[3, 11] = -np.inf
+    if profile == "fp32":
+        f[4, channels - 1] = 1e20
+        x[5, 0] = 1e20
+    gamma = rng.uniform(0.5, 1.5, channels).astype(np.float32)
+
+    def run(x, f, post, pre):
+        n, skip = x.size, int(unaligned)
+        bufs = [torch.zeros(n + skip, dtype=dt, device="cuda") for _ in range(4)]
+        for b, v in zip(bufs, (x, f)):
+            b[skip:] = torch.from_numpy(v).cuda().flatten()
+        beta = torch.full((channels,), 0.25, device="cuda")
+        d = dict(label="n", input=bufs[0][skip:], block=bufs[1][skip:], output=bufs[2][skip:], normalized=bufs[3][skip:],
+                 rows=x.shape[0], channels=channels, post=post, pre=pre)
+        for at, kind in (("post", post), ("pre", pre)):
+            d[at + "_gamma"] = torch.from_numpy(gamma).cuda()
+            if kind == "layer":
+                d[at + "_beta"] = beta
+        pk.kernels.ResidualNormKernel.create(device, None, 0, profile).create_dispatch(d).encode()
+        torch.cuda.synchronize()
+        return [b[skip:].cpu().numpy().reshape(x.shape) for b in bufs[2:]]
+
+    y, h = run(x, f, "rms", "rms")
+    rest = lambda row, at: np.delete(row, at)  # noqa: E731
+    # Row 1: u is 0 but for the infinite channel, so y is the input itself there; the pre norm of a row with NaN is NaN.
+    assert np.isnan(y[1, 7]) and np.array_equal(rest(y[1], 7), rest(x[1], 7)) and np.isnan(h[1]).all()
+    # Row 3: y has an infinite channel; h is 0 elsewhere.
+    assert np.isneginf(y[3, 11]) and np.isnan(h[3, 11]) and np.isfinite(rest(y[3], 11)).all() and not rest(h[3], 11).any()
+    if profile == "fp32":
+        assert np.array_equal(y[4], x[4]) and np.isfinite(h[4]).all() and h[4].any()
+        assert np.isfinite(y[5]).all() and not h[5].any()
+    yl, hl = run(x, f, "layer", "layer")
+    assert np.isnan(yl[1]).all() and np.isnan(hl[1]).all()  # inf - inf in the centred values
+    if profile == "fp32":
+        # The mean of row 4 is 1e20 / channels; what is left of the others' squares does not count.
+        assert np.array_equal(yl[4], x[4] + np.float32(0.25)) and np.array_equal(hl[5], np.full(channels, 0.25, np.float32))
+    keep = [0, 2] if profile == "fp32" else [0, 2, 4, 5]
+    for got, want in zip((y, h, yl, hl), run(x[keep], f[keep], "rms", "rms") + run(x[keep], f[keep], "layer", "layer")):
+        np.testing.assert_array_equal(got[keep], want)
