@@ -65,8 +65,10 @@ __device__ __forceinline__ float i4_lds_f32(uint32_t addr) {
 
 // Eight inputs of a row as f16 columns, in the order 0 4 1 5 2 6 3 7 in which a
 // word of codes gives its pairs; 16 lanes (`mask`) hold a tile's 128.  FP32: two
-// columns and the factor `down` that undoes their scale.  Returns whether an
-// input was infinite or NaN; it becomes 0.
+// columns and the factor `down` that undoes their scale where it is applied
+// twice, once to the weights' scale and once to the sum: the whole of it would
+// take either out of f32's range where the product is well inside.  Returns
+// whether an input was infinite or NaN; it becomes 0.
 template <typename T>
 __device__ __forceinline__ bool i4_columns(const uint4 (&raw)[sizeof(T) / 2], uint32_t mask, uint4 (&col)[sizeof(T) / 2],
                                            float& down) {
@@ -103,10 +105,10 @@ __device__ __forceinline__ bool i4_columns(const uint4 (&raw)[sizeof(T) / 2], ui
     }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
-    // 2^s with the largest magnitude in [2^14, 2^15); s <= 126 keeps 2^s and 2^-s normal.
-    const int s = min(141 - (int)(top >> 23), 126);
+    // 2^s with the largest magnitude in [2^13, 2^15), s even; s <= 126 keeps 2^s normal.
+    const int s = min(141 - (int)(top >> 23), 126) & ~1;
     const float up = __uint_as_float((uint32_t)(s + 127) << 23);
-    down = __uint_as_float((uint32_t)(127 - s) << 23);
+    down = __uint_as_float((uint32_t)(127 - s / 2) << 23);
     __half hi[8], lo[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

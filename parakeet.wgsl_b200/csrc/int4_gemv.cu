@@ -28,7 +28,7 @@
 // The scale multiplies a group's f32 sum, not the weight: no weight is
 // rounded.  FP32 rows are two f16 columns each, the leading 11 bits and the
 // next 11, after a power-of-two scale per row and 128 inputs that brings the
-// largest to [2^14, 2^15): 22 bits of every input, where the sum's own rounding
+// largest to [2^13, 2^15): 22 bits of every input, where the sum's own rounding
 // is 24.  An infinite or NaN input is laid out as 0 and its row marked; the
 // thread that joins such a row's sum adds those products itself, from A.
 //
@@ -306,6 +306,10 @@ __global__ void __launch_bounds__(i4_warps(NT) * 32, 1) int4_gemv_kernel(const I
 #pragma unroll
               for (int m = 0; m < MT; ++m) {
                 const float f0 = PARTS == 2 ? s0[m] * f : s0[m], f1 = PARTS == 2 ? s1[m] * f : s1[m];
+                if constexpr (PARTS == 2) {
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) acc[m][n][e] *= f;
+                }
                 total[m][n][0] = fmaf(f0, acc[m][n][0], total[m][n][0]);
                 total[m][n][1] = fmaf(f0, acc[m][n][1], total[m][n][1]);
                 total[m][n][2] = fmaf(f1, acc[m][n][2], total[m][n][2]);

@@ -411,11 +411,17 @@ __global__ void __launch_bounds__(IU_THREADS, 1) int4_umma_kernel(const I4Params
 #pragma unroll
                 for (int r = 0; r < LD / 2; r += 4) {
                   const float4 f = *reinterpret_cast<const float4*>(xscale + kt * RP + c0 / 2 + r);
-                  const float fs[4] = {f.x, f.y, f.z, f.w};
+                  const float2 fs[2] = {make_float2(f.x, f.y), make_float2(f.z, f.w)};
 #pragma unroll
-                  for (int j = 0; j < 4; ++j)
-                    total[c0 / 2 + r + j] = fmaf(scale * fs[j], __uint_as_float(v[2 * (r + j)]) + __uint_as_float(v[2 * (r + j) + 1]),
-                                                 total[c0 / 2 + r + j]);
+                  for (int j = 0; j < 2; ++j) {  // two rows
+                    const uint32_t* w = v + 2 * r + 4 * j;
+                    float* to = total + c0 / 2 + r + 2 * j;
+                    const float2 u = make_float2(__uint_as_float(w[0]) + __uint_as_float(w[1]),
+                                                 __uint_as_float(w[2]) + __uint_as_float(w[3]));
+                    const float2 sum = ffma2(fmul2(make_float2(scale, scale), fs[j]), fmul2(u, fs[j]), make_float2(to[0], to[1]));
+                    to[0] = sum.x;
+                    to[1] = sum.y;
+                  }
                 }
               }
             }

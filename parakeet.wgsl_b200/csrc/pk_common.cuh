@@ -404,6 +404,14 @@ __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
         "l"(*reinterpret_cast<const uint64_t*>(&c)));
   return *reinterpret_cast<const float2*>(&d);
 }
+// Two products, rounded as a * b.
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
+  return *reinterpret_cast<const float2*>(&d);
+}
 
 // -------------------------------------------------------------- math bits
 // SiLU exactly as the reference epilogue writes it:

@@ -165,3 +165,40 @@ def test_residual_norm_of_rows_whose_squares_leave_f32(pk, device, profile, chan
     keep = [0, 2] if profile == "fp32" else [0, 2, 4, 5]
     for got, want in zip((y, h, yl, hl), run(x[keep], f[keep], "rms", "rms") + run(x[keep], f[keep], "layer", "layer")):
         np.testing.assert_array_equal(got[keep], want)
+
+
+# ====================================================================== int4 products
+
+# mma.sync (one and two column tiles, four in two passes) and tcgen05 (16 and 32 columns, groups of every kind).
+@pytest.mark.parametrize("rows,inner,columns,group", [
+    (1, 640, 640, 64), (5, 512, 48, 128), (12, 1024, 200, 32), (17, 640, 19000, 64), (10, 4096, 6000, 128),
+    (40, 1056, 12005, 32),
+])
+@pytest.mark.parametrize("inputs,weights", [(1e-34, 1.0), (1e-37, 1.0), (1e-20, 1e-17), (1e-38, 1e3), (1e35, 1.0), (1e37, 1e-4),
+                                            (1e30, 1e6), (1.0, 1e-30), (1.0, 1e33)])
+def test_int4_gemv_of_small_and_large_numbers(pk, device, rows, inner, columns, group, inputs, weights):
+    """FP32 inputs and scales near the ends of the type: as near to the formula as those near one, as far as f32
+    has numbers for the products."""
+    import torch
+
+    rng = np.random.default_rng(rows + inner)
+    codes = rng.integers(0, 16, (inner, columns)).astype(np.uint8)
+    scales = ((0.5 + rng.random((inner // group, columns))) * 0.05 * weights).astype(np.float32)
+    a = (rng.standard_normal((rows, inner)) * inputs).astype(np.float32)
+    out = torch.zeros((rows, columns), device="cuda")
+    weight = pk.kernels.Int4Weight.from_words(torch.from_numpy(pk.runtime_plan.pack_int4(codes).view(np.int32)).cuda(),
+                                              torch.from_numpy(scales).cuda(), inner, group)
+    pk.kernels.Int4GemvKernel.create(device, None, 0, "fp32").create_dispatch(dict(
+        label="g", a=torch.from_numpy(a).cuda(), weight=weight, output=out, rows=rows)).encode()
+    got = out.double().cpu().numpy()
+    w = (codes.astype(np.float64) - 8.0) * np.repeat(scales.astype(np.float64), group, axis=0)
+    a64 = a.astype(np.float64)
+    v, mass = a64 @ w, np.abs(a64) @ np.abs(w)
+    assert np.abs(v).max() < 1e38  # sums of terms of both signs: none on the way leaves f32
+    # f32 accumulation, up to one step (2^-23) per product instruction and join; inputs as two f16 parts lose at most
+    # 2^-22 of each and, relative to a tile's largest, 2^-38.  A product instruction's or group's sum below the
+    # smallest numbers is off by half a step of 2^-149.
+    dv = (inner / 16 + 64) * 2 * E * mass + 2.0 ** -22 * mass + 2.0 ** -38 * np.abs(a64).max() * np.abs(w).sum(axis=0)
+    dv = dv + (inner / 16 + 64) * 2.0 ** -150
+    err = np.abs(got - v) - dv * (1 + E) - E * np.abs(v)
+    assert np.all(err <= 0), (float(err.max()), float(np.abs(got - v).max()), float(np.abs(v).max()))
