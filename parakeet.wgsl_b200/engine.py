@@ -192,7 +192,7 @@ class ParakeetEngine:
         host["done"].synchronize()
         tok, fr, du = (host["tokens"][k, :b].numpy() for k in range(3))
         counts = host["meta"][:b].numpy()
-        flags = host["meta"][self.capacity:self.capacity + b].numpy()
+        flags = host["meta"][b:2 * b].numpy()  # the decoder's layout follows the batch, not the capacity
         out = []
         for i in range(b):
             n = min(int(counts[i]), self.max_tokens)
