@@ -49,7 +49,7 @@ def flags(verbose: bool = False) -> list[str]:
 def _compile(src: Path, verbose: bool) -> tuple[Path, str]:
     obj = BUILD / (src.stem + ".o")
     if obj.exists() and obj.stat().st_mtime > max(
-        [src.stat().st_mtime] + [h.stat().st_mtime for h in CSRC.glob("*.h*")]
+        [src.stat().st_mtime] + [h.stat().st_mtime for pattern in ("*.h", "*.cuh") for h in CSRC.glob(pattern)]
         + [(PKG.parent / "include" / "pk_b200.h").stat().st_mtime]
     ) and not verbose:
         return obj, ""
