@@ -770,12 +770,12 @@ class TokenScoresKernel:
             raise RangeError(f"{label} rows of {columns} columns from {first} do not fit a stride of {stride}")
         if k > 32 or k > columns:
             raise RangeError(f"{label} top_k must be in [0, 32] and at most {columns}, got {k}")
-        if "row_map" not in d and slots < rows:
+        if d.get("row_map") is None and slots < rows:
             raise RangeError(f"{label} outputs hold {slots} of {rows} rows")
         f32 = torch.float32
         logits = _operand(d, "logits", _scalar_dtype(self.profile), (rows - 1) * stride + first + columns, self.device)
         dev = self.device
-        targets = _operand(d, "targets", _ids(), slots, dev, optional="log_probs" not in d)
+        targets = _operand(d, "targets", _ids(), slots, dev, optional=d.get("log_probs") is None)
         outs = {n: _operand(d, n, f32, slots, dev, optional=True) for n in ("log_probs", "log_sums", "entropies")}
         outs["top_ids"] = _operand(d, "top_ids", _ids(), slots * k, dev, optional=True)
         outs["top_log_probs"] = _operand(d, "top_log_probs", f32, slots * k, dev, optional=True)

@@ -202,3 +202,23 @@ def test_int4_gemv_of_small_and_large_numbers(pk, device, rows, inner, columns, 
     dv = dv + (inner / 16 + 64) * 2.0 ** -150
     err = np.abs(got - v) - dv * (1 + E) - E * np.abs(v)
     assert np.all(err <= 0), (float(err.max()), float(np.abs(got - v).max()), float(np.abs(v).max()))
+
+
+# ====================================================================== optional operands
+
+def test_token_scores_take_none_for_what_is_not_wanted(pk, device):
+    """None stands for an output or operand that is left out, as the key's absence does."""
+    import torch
+
+    x = torch.randn(3, 100, device="cuda")
+    kernel = pk.kernels.TokenScoresKernel.create(device, None, 0, "fp32")
+    outs = [torch.zeros(3, device="cuda") for _ in range(2)]
+    left_out = dict(log_probs=None, targets=None, entropies=None, top_ids=None, top_log_probs=None, row_count=None, row_map=None)
+    for out, extra in zip(outs, ({}, left_out)):
+        kernel.create_dispatch(dict(label="s", logits=x, rows=3, columns=100, log_sums=out, **extra)).encode()
+    torch.cuda.synchronize()
+    assert torch.equal(*outs) and torch.isfinite(outs[0]).all()
+    with pytest.raises(pk.kernels.ParakeetError, match="needs targets"):
+        kernel.create_dispatch(dict(label="s", logits=x, rows=3, columns=100, log_probs=outs[0], targets=None))
+    with pytest.raises(pk.kernels.RangeError, match="outputs hold"):
+        kernel.create_dispatch(dict(label="s", logits=x, rows=3, columns=100, log_sums=outs[0], slots=2, row_map=None))
