@@ -338,7 +338,8 @@ int pk_int4_gemv(pk_device* device, const pk_int4_gemv_desc* desc, pk_stream str
  * hidden to f16, as the decoder does.  row_map[r] = w * max_tokens + u and
  * row_count are what pk_token_scores takes.  Rows behind the last are left as
  * they are.  Frames >= frames are read as frames - 1.  FP32 products are sums of three
- * in shorter parts: an infinite hidden value or weight makes NaN. */
+ * in shorter parts (22 bits of a value from 2^-115 on): an infinite hidden value or
+ * weight makes NaN. */
 typedef struct pk_joint_logits_desc {
   int precision;                 /* PK_FP16: encoder, weight, logits f16; PK_FP32: f32 */
   int batch, frames, max_tokens;

@@ -33,9 +33,10 @@
 // thread that joins such a row's sum adds those products itself, from A.
 //
 // 1x4096x65536 f16 26.7 us, 5.2 TB/s or 80% of a copy's rate; 8 rows 29.9 us (72%);
-// 1x4096x16384 f16 10.1 us and 1x640x640 f16 3.0 us, where start and join show.
-// 16 rows take 51 us: two MMAs a weight tile, and twice the columns to read from
-// shared memory.  (What marks infinite inputs costs 0.1 to 0.4 us of these.)
+// 1x4096x16384 f16 10.1 us and 1x640x640 f16 3.0 us (3.2 launched one by one),
+// where start and join show.  FP32: 1x4096x65536 27.4 us (80%), 4 rows 29.5, 8 rows
+// 46; 1x4096x16384 10.4 us.  16 columns (16 rows f16 51 us): two MMAs a weight
+// tile, and twice the columns to read from shared memory.  (What marks infinite inputs costs 0.1 to 0.4 us of these.)
 //
 // One CTA per SM walks the output tiles; A's rows are laid out in its shared
 // memory once.  Its warps split outputs (wm) and inputs (wk), so that the
@@ -412,8 +413,11 @@ int launch_typed(const DeviceCtx& dev, I4Params p, int group, cudaStream_t strea
     nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
     const int mt = i4_mt(nt);
     mgroups = (mtiles + mt - 1) / mt;
-    // Few tiles per SM: fewer warps to start and to join (8x4096x4096 f16 7.3 us
-    // with 20 against 8.0; at 221 tiles per SM, 1x4096x16384, 12.2 against 10.1).
+    // Few tiles per SM: fewer warps to start and to join.  With 4096 inputs 20 warps
+    // gain up to 138 tiles per SM (8x4096xN f16: 55 tiles 7.1 us against 7.8 with 28,
+    // 111 9.2 against 9.5, 138 9.9 against 10.7) and lose from 166 on (11.9 against
+    // 10.8; 221 18.3 against 11.9); with few inputs they lose earlier (8x640x32768, 69
+    // tiles, 8.3 against 7.0; 8x1024x32768, 111, 10.5 against 8.0).
     const int warps = nt == 1 && (int64_t)mgroups * p.ktiles < 100 * dev.sm_count ? 20 : i4_warps(nt);
     for (p.cluster = 1; p.cluster <= I4_CLUSTER; p.cluster *= 2) {
       // Few outputs: the inputs over more SMs, while each has a tile for every warp of 4.

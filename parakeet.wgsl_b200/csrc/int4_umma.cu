@@ -17,10 +17,14 @@
 // and four for the epilogue, each place of it owned by one of them.
 //
 // 16x4096x65536 f32 59 us (mma.sync 86), 32x4096x65536 f16 66 us (94); reading
-// the codes takes 21.  Bound by instructions: about 470 per tile of 128 x 128
-// and SM sub-partition, of which expanding is a third (without the expansion 53
-// us where it takes 58, f32 54 of 59; with an eighth of the copies 57; with an
-// eighth of the MMAs the same time).  Register loads instead of bulk copies kept one
+// the codes takes 21.  No part of it alone is the bound: a tile of 128 x 128 takes
+// about 1000 cycles, of which an SM sub-partition issues on 470 (a third of them
+// expand), and neither copies nor MMAs nor the expansion hold it up (without the
+// expansion 53 us where it takes 58, f32 54 of 59; with an eighth of the copies 57;
+// with an eighth of the MMAs the same time).  What is left is the chain of
+// hand-overs: a group of decode warps owns one stage of codes and one place in
+// TMEM, so that a copy, a store, an MMA and a commit follow one another before its
+// next tile.  Register loads instead of bulk copies kept one
 // tile on the way whatever the depth asked for (58 us with two groups of
 // decode warps); MMAs issued behind `lane == 0` instead of an elected lane took
 // 85 cycles each instead of 20.

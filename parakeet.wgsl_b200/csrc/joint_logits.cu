@@ -18,9 +18,9 @@
 // instructions (with one thread doing both between barriers a step took 2400
 // cycles, 900 of them the MMAs' issue and 800 the loads').
 //
-// 1 window (61 tokens, 640 x 1032) f16 8.4 us: 33 tiles, latency from start to
-// end.  32 windows f16 10.9 us: 144 tiles, one per SM; reading everything once
-// takes 2.  40 windows f32 48 us, bound by shared memory: a step of 32 inputs
+// 30 rows (1 window; 640 x 1032) f16 8.4 us: 33 tiles, latency from start to end.
+// 1531 rows (32 windows) f16 10.9 us: 144 tiles, one per SM, of which 12 gather the
+// same rows each; reading everything once takes 1.6.  3584 rows (40 windows) f32 48 us, bound by shared memory: a step of 32 inputs
 // writes 64 KB of split operands there, reads 96 KB of them for its MMAs and
 // moves 32 KB of weights in and out, 1540 of its 2100 cycles.
 //

@@ -13,8 +13,8 @@
 //
 // Bound by memory: two reads and two writes of every element, nothing in
 // between reaches memory.  16384x4096 f32 175 us, 6.1 TB/s or 94% of a copy's
-// rate; 16384x2048 f16 46 us, 5.9 TB/s; 6016x1024 f16 12.0 us; 1x640 f16 2.7 us,
-// a launch and one round trip.
+// rate; 16384x2048 f16 46 us, 5.9 TB/s; 6016x1024 f16 12.0 us; 1x640 f16 2.7 us
+// in a graph of such calls, 3.2 launched one by one: a launch and one round trip.
 //
 // Rows of up to 512 vectors of 16 bytes: a thread owns a vector's channels, keeps
 // their parameters in registers and takes four rows of its CTA at a time.  Longer

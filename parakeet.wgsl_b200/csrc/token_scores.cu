@@ -32,7 +32,8 @@
 // Bound by reading the logits once where rows are long and many, and there by
 // instructions on top: an element takes about ten (widen, compare, FMA, ex2, two
 // sums).  4096x50257 f16 100 us, 4.1 TB/s or 63% of a copy's rate (80 us without
-// alternatives); 16384x16384 f32 218 us, 4.9 TB/s.  Short calls are latency:
+// alternatives: the warps of a row meet, read their candidates again and load
+// nothing meanwhile); 16384x16384 f32 219 us, 4.9 TB/s.  Short calls are latency:
 // 1x32000 f16 5.7 us, 1953x1025 f32 6.4 us; a row of 8 columns takes 3.1.
 // A row belongs to one warp, to several
 // warps of a CTA or to a cluster of CTAs (joined through distributed shared
@@ -689,23 +690,23 @@ int launch_typed(const DeviceCtx& dev, const TsParams& p, cudaStream_t stream) {
   // More alternatives than half a warp's lanes: one warp's 32 lane maxima would bound them too loosely.
   const int64_t least = p.k > 16 ? 2 : 1;
   // Few rows: every warp holds little, over as many SMs as there are (1x32000 f16
-  // 6.3 us against 7.1 with TS_HELD vectors a lane and 8.6 streamed; 1x131072 9.1,
-  // 14.7 without a cluster).
+  // 5.7 us against 6.5 with TS_HELD vectors a lane and 7.7 streamed; 1x131072 8.4,
+  // 14.4 without a cluster).
   const int64_t few = std::max(warps_for(TS_HELD_FEW), least);
   if (few <= TS_WARPS * TS_CLUSTER && p.rows * few <= (int64_t)dev.sm_count * TS_WARPS)
     return launch_route<T, TS_HELD_FEW>(p, (int)std::min<int64_t>(few, TS_WARPS), (int)std::max<int64_t>(1, few / TS_WARPS),
                                         stream);
   // Rows that all run at once (two CTAs an SM): held, one round trip to memory
-  // (1000x4096 f16 8.4 us against 12.5 streamed, 1953x1025 f32 6.4 against 10.0).
+  // (1000x4096 f16 8.1 us against 12.3 streamed, 1953x1025 f32 6.4 against 10.2).
   // More rows are streamed, by warps that come and go with more of them on an SM
-  // (16384x4096 f16 51 us against 99 held, 4096x8192 23 against 53).
+  // (16384x4096 f16 50 us against 98 held, 4096x8192 22 against 51).
   const int64_t held = std::max(warps_for(TS_HELD), least);
   if (held <= TS_WARPS && p.rows * held <= 2 * (int64_t)dev.sm_count * TS_WARPS) return launch_route<T, TS_HELD>(p, (int)held, 1, stream);
   if (held <= TS_WARPS * TS_CLUSTER && p.rows * held <= (int64_t)dev.sm_count * TS_WARPS)
     return launch_route<T, TS_HELD>(p, TS_WARPS, (int)(held / TS_WARPS), stream);
-  // Streamed: a warp per row costs least (4096x8192 f16 23 us, 30 with two, 42 with
-  // four, 48 with eight), as long as the rows fill the SMs and those under way
-  // stay in L2, from where candidates are read again (4096x50257: 133, 129, 115, 105).
+  // Streamed: a warp per row costs least (4096x8192 f16 22 us, 30 with two, 41 with
+  // four, 46 with eight), as long as the rows fill the SMs and those under way
+  // stay in L2, from where candidates are read again (4096x50257: 133, 128, 114, 102).
   int cluster = 1;
   while (cluster < TS_CLUSTER && p.rows * cluster * 2 <= dev.sm_count) cluster *= 2;
   const int64_t warps = (int64_t)dev.sm_count * 4 * TS_WARPS;  // at once

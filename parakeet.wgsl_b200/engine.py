@@ -42,7 +42,11 @@ TOKEN_COLUMNS, DURATION_COLUMNS = 1025, 5  # of the joint's 1032 outputs, padded
 
 @dataclass(frozen=True)
 class EmissionScores:
-    """What the joint says about each of a window's emissions (natural logarithms, f32)."""
+    """What the joint says about each of a window's emissions (natural logarithms, f32).
+
+    The scores come from f32 sums over the decoder's own joint inputs.  The FP16
+    decoder takes its maximum over chains of f16 sums, as the reference does, so where
+    two tokens are close the emitted one need not be alternatives[:, 0]."""
     token_log_probs: np.ndarray      # [n] of the emitted token, among the 1025 tokens (blank included)
     duration_log_probs: np.ndarray   # [n] of the emitted duration, among the 5 durations
     token_entropies: np.ndarray      # [n] of the token distribution
@@ -65,7 +69,10 @@ class ParakeetEngine:
         """package: encoder + decoder tensors (name -> record), as produced by
         the reference converter or ``synthetic.make_package`` + ``make_decoder``.
         alternatives: when given, ``transcribe_windows`` scores every emission and
-        names its `alternatives` (0..32) most probable tokens."""
+        names its `alternatives` (0..32) most probable tokens.  The long-form calls
+        (``transcribe``, ``decode_plans``) return merged tokens and do not score.  The
+        scorer holds 4.6 KB of device memory (FP32 6.7) and 8 bytes per alternative for
+        each of capacity * max_tokens places, and copies a window's places back whole."""
         if alternatives is not None and not 0 <= alternatives <= 32:
             raise RangeError(f"alternatives must be in [0, 32], got {alternatives}")
         self.device, self.precision, self.capacity, self.max_tokens = device, precision, capacity, max_tokens
